@@ -5,7 +5,8 @@
  * This is the drop-in boundary for the reference's `ppocr_rs::gpu` direct
  * model API (src/gpu/mod.rs:3-13).  Every entry point names the reference
  * item it replaces.  Plain pointers and sizes only; no exception or abort
- * crosses it; the library owns all device memory.  A handle may be used from
+ * crosses it; the library owns all device memory (the operators on rows of
+ * logits alone work in the caller's).  A handle may be used from
  * any thread but not concurrently: forward calls serialise on a per-context
  * mutex, as the reference's `Mutex<SharedWorkspace>` does
  * (src/gpu/runtime.rs:75, :1753-1758).
@@ -345,6 +346,121 @@ ppocr_status ppocr_recognition_input_plan(const float corners[8], size_t input_w
 ppocr_status ppocr_ctc_greedy_decode(const float* steps, size_t time_steps, size_t classes, size_t dictionary_len,
                                      size_t content_width, size_t input_width, int32_t* tokens, size_t* n_tokens,
                                      float* score);
+
+/* ---- Operators on rows of class logits (no counterpart in the reference).
+ *
+ * A recognizer ends in one row of logits per time step.  These operators work
+ * on such rows in the caller's device memory, on the context's device: every
+ * pointer in them that is not null is device memory of that device.  The work
+ * is queued on `stream` (a hipStream_t of that device; NULL is HIP's default
+ * stream) and the call returns without waiting.  The operators allocate
+ * nothing, keep nothing between calls and need no workspace, so calls may run
+ * at once from several threads and streams and may be captured into graphs.
+ * The current device of the calling thread stays as it is.
+ *
+ * Row indices, classes and offsets that the device reads are checked there:
+ * those outside their range are left out as described.  Zero rows are no
+ * work.  Padding between rows is neither read nor written. */
+
+/* `rows` rows of `classes` logits, `stride` elements apart (stride >=
+ * classes), each element a float or a bfloat16 by `type`.  1 to 262144
+ * classes, up to 2097152 rows. */
+typedef struct ppocr_logits {
+  const void* data;
+  size_t rows, classes, stride;
+  ppocr_precision type;
+} ppocr_logits;
+
+/* Rules of the rows, each part optional (null pointers and zero counts).
+ *
+ * bias: tables of one float per class, added to the logits.  masks: tables of
+ * ceil(classes / 32) words whose bit c % 32 of word c / 32 tells whether class
+ * c is allowed.  row_bias and row_mask give each row's table; a negative index
+ * or one past the tables means none.  Without them a single table holds for
+ * all rows and as many tables as rows hold for one row each.
+ *
+ * history: the classes that each row has emitted, back to back, row r's at
+ * history_offsets[r] .. history_offsets[r + 1] - 1 (rows + 1 offsets, within
+ * history_len; classes outside the row's are left out).  A class that stands n
+ * > 0 times in it is penalised by the row's repetition (logits above 0 are
+ * divided by it, others multiplied), then by frequency * n + presence, which
+ * is subtracted.  Null penalties are neutral (1, 0, 0).
+ *
+ * Order: penalties, bias, mask.  A class that is not allowed becomes -inf
+ * whatever its logit is; a row whose mask allows nothing becomes all -inf.
+ * Every step rounds to fp32, the result once more to the logits' type. */
+typedef struct ppocr_logit_rules {
+  size_t classes; /* of the logits the rules are for */
+  const float* bias;
+  size_t n_bias;
+  const int32_t* row_bias;
+  const uint32_t* masks;
+  size_t n_masks;
+  const int32_t* row_mask;
+  const int32_t* history;
+  size_t history_len;
+  const int64_t* history_offsets;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+} ppocr_logit_rules;
+
+/* Applies `rules` to the rows and writes them to `out` (the same type, rows
+ * `out_stride` elements apart), which may be the logits themselves. */
+ppocr_status ppocr_hip_logit_rules(ppocr_hip_ctx* ctx, const ppocr_logits* logits, const ppocr_logit_rules* rules,
+                                   void* out, size_t out_stride, void* stream);
+
+/* The k best classes of each row (1 <= k <= 64) under `rules` (NULL: none),
+ * which are applied while the row is read: values [rows][k] fp32, largest
+ * first, and indices [rows][k].  Equal logits go to the lowest class; NaN
+ * comes before +inf; -inf is no candidate, and places without one hold -inf
+ * and -1.  `rest` [rows] (or NULL) receives log(sum of exp(logit /
+ * temperature)) over all other classes, -inf where there are none.  The
+ * values are not divided by the temperature (0.001 to 1000). */
+ppocr_status ppocr_hip_top_logits(ppocr_hip_ctx* ctx, const ppocr_logits* logits, const ppocr_logit_rules* rules,
+                                  size_t k, float temperature, float* values, int32_t* indices, float* rest,
+                                  void* stream);
+
+/* A teacher's rows as ppocr_hip_top_logits leaves them: values and indices
+ * [rows][k] (1 <= k <= 64), rest [rows] at the temperature of the loss, or
+ * NULL when the teacher's other classes count as impossible.  An entry counts
+ * when its index is one of the student's classes, its value is not -inf and no
+ * entry before it that counts has the same class.  A row without such an entry
+ * has no target: its loss and gradient are 0 and its logits are not looked at. */
+typedef struct ppocr_teacher {
+  const float* values;
+  const int32_t* indices;
+  const float* rest;
+  size_t k;
+} ppocr_teacher;
+
+/* Distillation loss of each row of the student's logits, and what its
+ * gradient needs.  With q the softmax of the teacher's values / temperature
+ * and rest, and p the student's softmax of logits / temperature, whose classes
+ * that are no entry form one bucket as the teacher's rest does:
+ *   loss = temperature^2 * sum over entries and rest of q (log q - log p),
+ * terms of q = 0 being 0.  `loss` is [rows]; `state` [rows][4] (or NULL): the
+ * largest logit, the sum of exp((logit - largest) / temperature), and the same
+ * two over the classes that are no entry; zeros without a target.  A row whose
+ * logits are all -inf has an infinite loss and no gradient (0); NaN and +inf
+ * among a row's logits make its loss and gradient NaN or infinite. */
+ppocr_status ppocr_hip_distill_loss(ppocr_hip_ctx* ctx, const ppocr_logits* student, const ppocr_teacher* teacher,
+                                    float temperature, float* loss, float* state, void* stream);
+
+/* Gradient of sum(grad_loss * loss) by the student's logits, from the `state`
+ * that ppocr_hip_distill_loss left for the same student, teacher and
+ * temperature.  `grad_loss` is [rows] or NULL (ones); `grad` is of the
+ * student's type, rows `grad_stride` elements apart, and may be the student's
+ * logits themselves. */
+ppocr_status ppocr_hip_distill_grad(ppocr_hip_ctx* ctx, const ppocr_logits* student, const ppocr_teacher* teacher,
+                                    const float* state, float temperature, const float* grad_loss, void* grad,
+                                    size_t grad_stride, void* stream);
+
+/* Loss and gradient in one call, with each logit read once where a row fits
+ * the registers of a workgroup. */
+ppocr_status ppocr_hip_distill(ppocr_hip_ctx* ctx, const ppocr_logits* student, const ppocr_teacher* teacher,
+                               float temperature, const float* grad_loss, float* loss, void* grad, size_t grad_stride,
+                               void* stream);
 
 #ifdef __cplusplus
 }

@@ -736,6 +736,8 @@ void enqueue_forward_image(ppocr_hip_model* model, const ppocr_hip_image* image,
   }
 }
 
+int context_device(const ppocr_hip_ctx* ctx) { return ctx->device; }
+
 void sync_context(ppocr_hip_ctx* ctx) {
   HIP_OK(hipSetDevice(ctx->device));
   HIP_OK(hipStreamSynchronize(ctx->stream));

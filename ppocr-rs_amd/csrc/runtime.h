@@ -172,6 +172,8 @@ ppocr_db_options db_options(const ppocr_db_options* o);
 size_t packet_bytes(size_t n);
 void enqueue_forward_image(ppocr_hip_model* model, const ppocr_hip_image* image, const float* corners,
                            const size_t* content_w, size_t n, char* packet, float* out, size_t out_cap);
+// HIP device of a context.
+int context_device(const ppocr_hip_ctx* ctx);
 // Waits for all work queued on the context's stream.
 void sync_context(ppocr_hip_ctx* ctx);
 

@@ -42,6 +42,8 @@ EXPORTS = (
     "ppocr_hip_db_postprocess", "ppocr_hip_db_postprocess_static", "ppocr_hip_detect", "ppocr_hip_detect_image", "ppocr_engine_default_options",
     "ppocr_hip_engine_load", "ppocr_hip_engine_free", "ppocr_hip_engine_recognize", "ppocr_ocr_result_lines",
     "ppocr_ocr_result_tokens", "ppocr_ocr_result_sizes", "ppocr_ocr_result_free",
+    "ppocr_hip_logit_rules", "ppocr_hip_top_logits", "ppocr_hip_distill_loss", "ppocr_hip_distill_grad",
+    "ppocr_hip_distill",
 )
 
 
@@ -138,6 +140,30 @@ class KernelStat(ctypes.Structure):
                 ("flops", ctypes.c_double), ("bytes", ctypes.c_double), ("bound", ctypes.c_int)]
 
 
+class _Logits(ctypes.Structure):
+    """``ppocr_logits``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_size_t), ("classes", ctypes.c_size_t),
+                ("stride", ctypes.c_size_t), ("type", ctypes.c_int)]
+
+
+class _Rules(ctypes.Structure):
+    """``ppocr_logit_rules``."""
+
+    _fields_ = [("classes", ctypes.c_size_t),
+                ("bias", ctypes.c_void_p), ("n_bias", ctypes.c_size_t), ("row_bias", ctypes.c_void_p),
+                ("masks", ctypes.c_void_p), ("n_masks", ctypes.c_size_t), ("row_mask", ctypes.c_void_p),
+                ("history", ctypes.c_void_p), ("history_len", ctypes.c_size_t), ("history_offsets", ctypes.c_void_p),
+                ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p)]
+
+
+class _Teacher(ctypes.Structure):
+    """``ppocr_teacher``."""
+
+    _fields_ = [("values", ctypes.c_void_p), ("indices", ctypes.c_void_p), ("rest", ctypes.c_void_p),
+                ("k", ctypes.c_size_t)]
+
+
 _lib = None
 _SZ = ctypes.POINTER(ctypes.c_size_t)
 _F = ctypes.POINTER(ctypes.c_float)
@@ -193,6 +219,12 @@ def lib():
         L.ppocr_hip_detect.argtypes = [_VP, _F, ctypes.c_size_t, _T, _O, _D8, ctypes.c_size_t, _SZ, _SZ]
         L.ppocr_hip_detect_image.argtypes = [_VP, _VP, _F, ctypes.c_size_t, _T, _O, _D8, ctypes.c_size_t, _SZ,
                                              _SZ]
+        _LG, _RU, _TE = ctypes.POINTER(_Logits), ctypes.POINTER(_Rules), ctypes.POINTER(_Teacher)
+        L.ppocr_hip_logit_rules.argtypes = [_VP, _LG, _RU, _VP, ctypes.c_size_t, _VP]
+        L.ppocr_hip_top_logits.argtypes = [_VP, _LG, _RU, ctypes.c_size_t, ctypes.c_float, _VP, _VP, _VP, _VP]
+        L.ppocr_hip_distill_loss.argtypes = [_VP, _LG, _TE, ctypes.c_float, _VP, _VP, _VP]
+        L.ppocr_hip_distill_grad.argtypes = [_VP, _LG, _TE, _VP, ctypes.c_float, _VP, _VP, ctypes.c_size_t, _VP]
+        L.ppocr_hip_distill.argtypes = [_VP, _LG, _TE, ctypes.c_float, _VP, _VP, _VP, ctypes.c_size_t, _VP]
         _lib = L
     return _lib
 
@@ -223,6 +255,140 @@ class ModelOutput:
         return self.values.reshape(self.shape)
 
 
+# ------------------------------------------------- operators on rows of logits
+
+_torch_module = None
+
+
+def _torch():
+    """torch, whose tensors the operators take (nothing else here needs it).
+    Its memory and streams belong to the HIP runtime that it loaded; a second
+    one in the process, loaded by this library before torch, cannot use them."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        lib()
+        with open("/proc/self/maps") as maps:
+            found = {line.split()[-1] for line in maps if "libamdhip64" in line}
+        if len(found) > 1:
+            raise RuntimeError("two HIP runtimes are loaded: import torch before the first call into this library")
+        _torch_module = torch
+    return _torch_module
+
+
+def _rows(t, what):
+    """``ppocr_logits`` of a tensor [..., classes] whose rows lie one stride apart."""
+    if t.dim() < 1:
+        raise ValueError(f"{what} needs a dimension of classes")
+    if t.dim() != 2:
+        t = t.view(-1, t.shape[-1])  # raises where the rows are not one stride apart
+    rows, classes = t.shape
+    if classes > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: the classes of a row must be adjacent")
+    kind = str(t.dtype)
+    if kind not in ("torch.float32", "torch.bfloat16"):
+        raise ValueError(f"{what} must be float32 or bfloat16, not {kind}")
+    return _Logits(t.data_ptr(), rows, classes, t.stride(0) if rows > 1 else max(classes, t.stride(0)),
+                   1 if kind == "torch.bfloat16" else 0)
+
+
+def _rows_like(t, like, what):
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{what} must have the logits' shape and type")
+    return _rows(t, what)
+
+
+def _packed(t, dtype, count, what):
+    """Pointer of a contiguous tensor of ``count`` elements (None: None)."""
+    if t is None:
+        return None
+    if str(t.dtype) != "torch." + dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor")
+    if count is not None and t.numel() != count:
+        raise ValueError(f"{what} has {t.numel()} elements, needs {count}")
+    return t.data_ptr()
+
+
+@dataclass
+class TopLogits:
+    """The k best classes of rows of logits: values [..., k] (float32), indices
+    [..., k] (int32; -1 with the value -inf where there are fewer), and rest
+    [...], the log-sum-exp of the other classes at the temperature it was asked
+    for.  As a teacher, ``rest`` may be None: no other class is possible."""
+
+    values: object
+    indices: object
+    rest: object = None
+
+
+def _teacher(t, rows):
+    if t.values.dim() < 1 or t.values.shape != t.indices.shape:
+        raise ValueError("the teacher's values and indices must have one shape [..., k]")
+    k = t.values.shape[-1]
+    return _Teacher(_packed(t.values, "float32", rows * k, "the teacher's values"),
+                    _packed(t.indices, "int32", rows * k, "the teacher's indices"),
+                    _packed(t.rest, "float32", rows, "the teacher's rest"), k)
+
+
+def class_masks(allowed):
+    """Mask words [n, ceil(classes / 32)] (int32) of a boolean tensor [n, classes]
+    of allowed classes."""
+    torch = _torch()
+    n, classes = allowed.shape
+    bits = torch.zeros((n, -(-classes // 32) * 32), dtype=torch.int64, device=allowed.device)
+    bits[:, :classes] = allowed
+    weights = torch.ones(32, dtype=torch.int64, device=allowed.device) << torch.arange(32, device=allowed.device)
+    words = (bits.reshape(n, -1, 32) * weights).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+class LogitRules:
+    """Rules on rows of ``classes`` logits (``ppocr_logit_rules``); every part
+    is optional.  The tensors are kept and read by each call, so a program may
+    change them in place between calls.
+
+    bias [n, classes] float32 and masks [n, ceil(classes / 32)] int32 words
+    (``class_masks``), with row_bias and row_mask [rows] int32 giving each row's
+    table (negative: none); without an index, one table for all rows or one a
+    row.  history (int32 classes back to back) with history_offsets [rows + 1]
+    int64, and repetition, frequency and presence [rows] float32."""
+
+    def __init__(self, classes, bias=None, row_bias=None, masks=None, row_mask=None, history=None,
+                 history_offsets=None, repetition=None, frequency=None, presence=None):
+        s = _Rules(classes=int(classes))
+        self._kept = (bias, row_bias, masks, row_mask, history, history_offsets, repetition, frequency, presence)
+        self._counts = []
+        if bias is not None:
+            if bias.dim() != 2 or bias.shape[1] != classes:
+                raise ValueError("bias must be [n, classes]")
+            s.bias, s.n_bias = _packed(bias, "float32", None, "bias"), bias.shape[0]
+        if masks is not None:
+            if masks.dim() != 2 or masks.shape[1] != -(-int(classes) // 32):
+                raise ValueError("masks must be [n, ceil(classes / 32)] words")
+            s.masks, s.n_masks = _packed(masks, "int32", None, "masks"), masks.shape[0]
+        if history is not None:
+            s.history, s.history_len = _packed(history, "int32", None, "history"), history.numel()
+        s.row_bias = self._row(row_bias, "int32", 0, "row_bias")
+        s.row_mask = self._row(row_mask, "int32", 0, "row_mask")
+        s.history_offsets = self._row(history_offsets, "int64", 1, "history_offsets")
+        s.repetition = self._row(repetition, "float32", 0, "repetition")
+        s.frequency = self._row(frequency, "float32", 0, "frequency")
+        s.presence = self._row(presence, "float32", 0, "presence")
+        self.struct = s
+
+    def _row(self, t, dtype, extra, what):
+        if t is not None:
+            self._counts.append((t.numel() - extra, what))
+        return _packed(t, dtype, None, what)
+
+    def check(self, rows):
+        """Raises unless every per-row part is for ``rows`` rows."""
+        for n, what in self._counts:
+            if n != rows:
+                raise ValueError(f"{what} is for {n} rows, the logits have {rows}")
+
+
 class Gpu:
     """``gpu::Gpu`` (src/gpu/runtime.rs:94-229): one device, stream and arena."""
 
@@ -230,6 +396,7 @@ class Gpu:
         h = _VP()
         _check(lib().ppocr_hip_create(int(device), ctypes.byref(h)))
         self.handle = h
+        self.device = int(device)
         self._children = []
 
     def info(self):
@@ -286,6 +453,80 @@ class Gpu:
         o = db_options(**options)
         return _collect(lambda buf, cap, counts, total: lib().ppocr_hip_db_postprocess_static(
             self.handle, p.ctypes.data_as(_F), n, h, w, tr, ctypes.byref(o), buf, cap, counts, total), n, o.max_boxes)
+
+    # Operators on rows of class logits: torch tensors on this device, the
+    # work queued on torch's current stream of the device.
+
+    def _stream(self):
+        return _torch().cuda.current_stream(self.device).cuda_stream
+
+    def logit_rules(self, logits, rules, out=None):
+        """Penalties, biases and masks of ``rules`` (LogitRules) on logits
+        [..., classes] (float32 or bfloat16); ``out`` may be the logits."""
+        rows = _rows(logits, "logits")
+        rules.check(rows.rows)
+        if out is None:
+            out = _torch().empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        o = _rows_like(out, logits, "out")
+        _check(lib().ppocr_hip_logit_rules(self.handle, rows, rules.struct, o.data, o.stride, self._stream()))
+        return out
+
+    def top_logits(self, logits, k, rules=None, temperature=1.0):
+        """The k best classes of each row and the log-sum-exp of the others at
+        ``temperature``, under ``rules``: TopLogits of [..., k] and [...]."""
+        torch = _torch()
+        rows = _rows(logits, "logits")
+        if rules is not None:
+            rules.check(rows.rows)
+        lead = logits.shape[:-1]
+        values = torch.empty((*lead, int(k)), dtype=torch.float32, device=logits.device)
+        indices = torch.empty((*lead, int(k)), dtype=torch.int32, device=logits.device)
+        rest = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        _check(lib().ppocr_hip_top_logits(self.handle, rows, rules.struct if rules is not None else None, int(k),
+                                          temperature, values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
+                                          self._stream()))
+        return TopLogits(values, indices, rest)
+
+    def distill_loss(self, student, teacher, temperature=1.0):
+        """Loss [...] of each row of the student's logits against ``teacher``
+        (TopLogits), and the state [..., 4] that ``distill_grad`` takes."""
+        torch = _torch()
+        rows = _rows(student, "student")
+        t = _teacher(teacher, rows.rows)
+        lead = student.shape[:-1]
+        loss = torch.empty(lead, dtype=torch.float32, device=student.device)
+        state = torch.empty((*lead, 4), dtype=torch.float32, device=student.device)
+        _check(lib().ppocr_hip_distill_loss(self.handle, rows, t, temperature, loss.data_ptr(), state.data_ptr(),
+                                            self._stream()))
+        return loss, state
+
+    def distill_grad(self, student, teacher, state, temperature=1.0, grad_loss=None, out=None):
+        """Gradient of ``sum(grad_loss * loss)`` by the student's logits, from
+        the state that ``distill_loss`` left; ``out`` may be the logits."""
+        rows = _rows(student, "student")
+        t = _teacher(teacher, rows.rows)
+        if out is None:
+            out = _torch().empty(student.shape, dtype=student.dtype, device=student.device)
+        o = _rows_like(out, student, "out")
+        _check(lib().ppocr_hip_distill_grad(self.handle, rows, t, _packed(state, "float32", rows.rows * 4, "state"),
+                                            temperature, _packed(grad_loss, "float32", rows.rows, "grad_loss"),
+                                            o.data, o.stride, self._stream()))
+        return out
+
+    def distill(self, student, teacher, temperature=1.0, grad_loss=None, out=None):
+        """Loss and gradient in one call: (loss [...], gradient); ``out`` may
+        be the student's logits."""
+        torch = _torch()
+        rows = _rows(student, "student")
+        t = _teacher(teacher, rows.rows)
+        loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=student.device)
+        if out is None:
+            out = torch.empty(student.shape, dtype=student.dtype, device=student.device)
+        o = _rows_like(out, student, "out")
+        _check(lib().ppocr_hip_distill(self.handle, rows, t, temperature,
+                                       _packed(grad_loss, "float32", rows.rows, "grad_loss"), loss.data_ptr(),
+                                       o.data, o.stride, self._stream()))
+        return loss, out
 
     def close(self):
         for child in self._children:
