@@ -56,19 +56,6 @@ __device__ __forceinline__ RowRules row_rules(const RuleParams& p, int64_t row, 
   return r;
 }
 
-// The rules on one logit, every step rounded to fp32 by itself.
-__device__ __forceinline__ float apply_rules(const RowRules& r, float x, int c, int n) {
-#pragma clang fp contract(off)
-  if (n > 0) {
-    x = x > 0.0f ? x / r.repetition : x * r.repetition;
-    const float f = r.frequency * (float)n;
-    x = x - (f + r.presence);
-  }
-  if (r.bias) x = x + r.bias[c];
-  if (r.mask && !(r.mask[c >> 5] >> (c & 31) & 1)) x = -INFINITY;
-  return x;
-}
-
 // Counts of the classes [first, first + n) in the row's history.
 __device__ __forceinline__ void count_history(const RowRules& r, int first, int n, int* counts) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
@@ -80,19 +67,145 @@ __device__ __forceinline__ void count_history(const RowRules& r, int first, int 
   __syncthreads();
 }
 
+// 16 bytes of a row: its elements as fp32, at any alignment of the element.
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+  static constexpr int N = 4;
+  typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const Raw r = *reinterpret_cast<const Raw*>(p);
+    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    *reinterpret_cast<Raw*>(p) = Raw{v[0], v[1], v[2], v[3]};
+  }
+};
+template <>
+struct Pack<bf16> {
+  static constexpr int N = 8;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
+  static __device__ __forceinline__ void load(const bf16* p, float (&v)[8]) {
+    const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float (&v)[8]) {
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<Raw*>(p) = r;
+  }
+};
+
+// The steps of the rules on one logit, every one rounded to fp32 by itself.
+__device__ __forceinline__ float penalise(const RowRules& r, float x, int n) {
+#pragma clang fp contract(off)
+  x = x > 0.0f ? x / r.repetition : x * r.repetition;
+  const float f = r.frequency * (float)n;
+  return x - (f + r.presence);
+}
+// Allowed classes c .. c + N - 1 (c a multiple of N) as N bits.
+template <int N>
+__device__ __forceinline__ unsigned mask_bits(const uint32_t* mask, int c) {
+  const unsigned b = reinterpret_cast<const uint8_t*>(mask)[c >> 3];
+  return N == 8 ? b : (b >> (c & 4)) & 15u;
+}
+__device__ __forceinline__ bool mask_bit(const uint32_t* mask, int c) { return mask[c >> 5] >> (c & 31) & 1; }
+
+__device__ __forceinline__ float apply_rules(const RowRules& r, float x, int c, int n) {
+  if (n > 0) x = penalise(r, x, n);
+  if (r.bias) x = x + r.bias[c];
+  return r.mask && !mask_bit(r.mask, c) ? -INFINITY : x;
+}
+
+// Rules of a chunk of one row: 16 elements a thread, each read and written
+// once, bound by HBM.  A pack without an allowed class is not read, and in
+// place one that no rule changes is neither read nor written.  Counts of the
+// history's classes in the chunk are an LDS histogram, so a chunk costs one
+// pass over the row's history (from L2 after the first chunk).
 constexpr int kChunk = 4096;
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, RuleParams p, T* out, int64_t out_stride) {
-  __shared__ int counts[kChunk];
+template <typename T, bool HISTORY>
+__global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, RuleParams p, T* out, int64_t out_stride,
+                                                               int chunk) {
+  constexpr int N = Pack<T>::N, PER = kChunk / (kThreads * N);
+  __shared__ int counts[HISTORY ? kChunk : 1];
   const int64_t row = blockIdx.x;
-  const int first = blockIdx.y * kChunk, n = min(kChunk, in.classes - first);
+  const int first = blockIdx.y * chunk, n = min(chunk, in.classes - first), tid = threadIdx.x;
   const RowRules r = row_rules(p, row, in.classes);
-  if (r.n_history) count_history(r, first, n, counts);
+  const bool counted = HISTORY && r.n_history > 0;
   const T* x = static_cast<const T*>(in.x) + row * in.stride + first;
   T* y = out + row * out_stride + first;
-  for (int i = threadIdx.x; i < n; i += kThreads)
-    st1<T>(y + i, apply_rules(r, ld1<T>(x + i), first + i, r.n_history ? counts[i] : 0));
+  const bool in_place = x == y && !r.bias;
+  const int full = n / N;
+  unsigned bits[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + j * kThreads;
+    bits[j] = (1u << N) - 1;
+    if (r.mask && i < full) bits[j] = mask_bits<N>(r.mask, first + i * N);
+  }
+  if (counted) count_history(r, first, n, counts);
+  float v[PER][N];
+  bool write[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + j * kThreads;
+    write[j] = i < full;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[j][e] = -INFINITY;
+    if (write[j] && in_place && bits[j] == (1u << N) - 1) {
+      write[j] = false;
+      if (counted)
+#pragma unroll
+        for (int e = 0; e < N; ++e) write[j] |= counts[i * N + e] > 0;
+    }
+    if (write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
+  }
+  if (counted)
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = tid + j * kThreads;
+      if (write[j] && bits[j])
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int c = counts[i * N + e];
+          if (c > 0) v[j][e] = penalise(r, v[j][e], c);
+        }
+    }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + j * kThreads;
+    if (!write[j]) continue;
+    if (r.bias && bits[j]) {
+      float b[N];
+      if constexpr (N == 4) {
+        Pack<float>::load(r.bias + first + i * N, b);
+      } else {
+        float lo[4], hi[4];
+        Pack<float>::load(r.bias + first + i * N, lo);
+        Pack<float>::load(r.bias + first + i * N + 4, hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = lo[e], b[4 + e] = hi[e];
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[j][e] = v[j][e] + b[e];
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (!(bits[j] >> e & 1)) v[j][e] = -INFINITY;
+    Pack<T>::store(y + i * N, v[j]);
+  }
+  // The last n % N classes, one a thread.
+  if (tid < n - full * N) {
+    const int i = full * N + tid;
+    st1<T>(y + i, apply_rules(r, ld1<T>(x + i), first + i, counted ? counts[i] : 0));
+  }
 }
 
 // A total order of (logit, class): larger is better.  NaN above all, -0 as +0,
@@ -355,13 +468,25 @@ __global__ __launch_bounds__(kThreads) void distill_grad_kernel(LogitRows s, Dis
 }  // namespace
 
 void launch_logit_rules(const LogitRows& in, const RuleParams& rules, void* out, int64_t out_stride, hipStream_t s) {
-  const dim3 grid((unsigned)in.rows, (unsigned)((in.classes + kChunk - 1) / kChunk));
-  if (in.dt == DT_BF16)
-    hipLaunchKernelGGL(logit_rules_kernel<bf16>, grid, dim3(kThreads), 0, s, in, rules, static_cast<bf16*>(out),
-                       out_stride);
-  else
-    hipLaunchKernelGGL(logit_rules_kernel<float>, grid, dim3(kThreads), 0, s, in, rules, static_cast<float*>(out),
-                       out_stride);
+  // Chunks of equal length (whole packs), at most kChunk classes.
+  const int n = (in.classes + kChunk - 1) / kChunk;
+  const int chunk = ((in.classes + n - 1) / n + 7) / 8 * 8;
+  const dim3 grid((unsigned)in.rows, (unsigned)((in.classes + chunk - 1) / chunk));
+#define RULES_LAUNCH(T, H)                                                                                          \
+  hipLaunchKernelGGL((logit_rules_kernel<T, H>), grid, dim3(kThreads), 0, s, in, rules, static_cast<T*>(out), \
+                     out_stride, chunk)
+  if (in.dt == DT_BF16) {
+    if (rules.history)
+      RULES_LAUNCH(bf16, true);
+    else
+      RULES_LAUNCH(bf16, false);
+  } else {
+    if (rules.history)
+      RULES_LAUNCH(float, true);
+    else
+      RULES_LAUNCH(float, false);
+  }
+#undef RULES_LAUNCH
 }
 
 void launch_top_logits(const LogitRows& in, const TopParams& p, hipStream_t s) {
