@@ -243,74 +243,407 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   for (int i = 1; i < (int)(blockDim.x >> 6); ++i) r += red[i];
   return r;
 }
+__device__ __forceinline__ double wave_sum(double v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  return v;
+}
 
-// k passes, each finding the best key below the last one.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void top_logits_kernel(LogitRows in, TopParams p) {
+// A part of a row in registers: PER packs a thread, pack j of thread t at
+// class first + (j * NT + t) * N, and one class of the row's last
+// classes % N (held with the first part; -inf elsewhere).
+template <typename T, int NT, int PER>
+struct RowPart {
+  static constexpr int N = Pack<T>::N;
+  static constexpr int kClasses = NT * PER * N;
+  float v[PER][N];
+  float tail;
+};
+
+// Reads part `seg` of a row, classes past the row -inf.
+template <typename T, int NT, int PER>
+__device__ __forceinline__ void load_part(RowPart<T, NT, PER>& d, const T* x, int classes, int seg) {
+  constexpr int N = Pack<T>::N;
+  const int full = classes / N;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+    if (i < full)
+      Pack<T>::load(x + i * N, d.v[j]);
+    else
+#pragma unroll
+      for (int e = 0; e < N; ++e) d.v[j][e] = -INFINITY;
+  }
+  d.tail = -INFINITY;
+  if (seg == 0 && (int)threadIdx.x < classes - full * N) d.tail = ld1<T>(x + full * N + threadIdx.x);
+}
+
+// The rules on a part in registers.  The history is counted in windows of
+// kWindow classes, whole rounds of packs.
+constexpr int kWindow = 8192;
+
+template <typename T, int NT, int PER>
+__device__ __forceinline__ void rule_part(RowPart<T, NT, PER>& d, const RowRules& r, int classes, int seg, int* counts) {
+  constexpr int N = Pack<T>::N, kRounds = kWindow / (NT * N);
+  static_assert(kRounds >= 1 && kWindow % (NT * N) == 0, "a window is whole rounds");
+  const int full = classes / N, tail = full * N + (int)threadIdx.x;
+  if (r.n_history) {
+    int tail_count = 0;
+#pragma unroll
+    for (int w = 0; w < PER; w += kRounds) {
+      const int first = (seg * PER + w) * NT * N;
+      if (first >= classes) break;
+      __syncthreads();  // the window before is no longer read
+      count_history(r, first, min(kWindow, classes - first), counts);
+      if (tail >= first && tail < min(first + kWindow, classes)) tail_count = counts[tail - first];
+#pragma unroll
+      for (int j = w; j < w + kRounds && j < PER; ++j) {
+        const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+        if (i < full)
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const int c = counts[i * N + e - first];
+            if (c > 0) d.v[j][e] = penalise(r, d.v[j][e], c);
+          }
+      }
+    }
+    // The row's last classes may lie in a window behind their part.
+    if (seg == 0 && tail < classes) {
+      if (tail >= PER * NT * N)
+        for (int i = 0; i < r.n_history; ++i) tail_count += r.history[i] == tail;
+      if (tail_count > 0) d.tail = penalise(r, d.tail, tail_count);
+    }
+  }
+  if (r.bias) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+      if (i < full)
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+          float b[4];
+          Pack<float>::load(r.bias + i * N + q, b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d.v[j][q + e] = d.v[j][q + e] + b[e];
+        }
+    }
+    if (seg == 0 && tail < classes) d.tail = d.tail + r.bias[tail];
+  }
+  if (r.mask) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+      const unsigned bits = i < full ? mask_bits<N>(r.mask, i * N) : 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (!(bits >> e & 1)) d.v[j][e] = -INFINITY;
+    }
+    if (seg == 0 && tail < classes && !mask_bit(r.mask, tail)) d.tail = -INFINITY;
+  }
+}
+
+template <typename T, int NT, int PER, bool RULES>
+__device__ __forceinline__ void read_part(RowPart<T, NT, PER>& d, const T* x, const RowRules& r, int classes, int seg,
+                                          int* counts) {
+  load_part(d, x, classes, seg);
+  if constexpr (RULES) rule_part(d, r, classes, seg, counts);
+}
+
+template <int N>
+__device__ __forceinline__ float pack_max(const float (&v)[N]) {
+  float m = v[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) m = fmaxf(m, v[e]);
+  return m;
+}
+
+// Wave sums of exp((x - max) * c) with their own maxima, joined over the parts
+// of a row: (m, s) becomes the sum of both.  -inf is no maximum.
+__device__ __forceinline__ void join_sums(float& m, double& s, float om, double os, float c) {
+  const float nm = fmaxf(m, om);
+  if (nm == -INFINITY) return;
+  s = (m == -INFINITY ? 0.0 : s * (double)__builtin_amdgcn_exp2f((m - nm) * c)) +
+      (om == -INFINITY ? 0.0 : os * (double)__builtin_amdgcn_exp2f((om - nm) * c));
+  m = nm;
+}
+
+// The sum of exp((v - m) * c) over a part, m the wave's maximum of it, limited to
+// finite numbers: +inf then counts as an infinite term and -inf as none.
+template <typename T, int NT, int PER>
+__device__ __forceinline__ void part_sum(const RowPart<T, NT, PER>& d, float c, float& m, double& sum) {
+  constexpr int N = Pack<T>::N;
+  float t = d.tail;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) t = fmaxf(t, pack_max(d.v[j]));
+  m = wave_max(t);
+  const float ref = fminf(fmaxf(m, -FLT_MAX), FLT_MAX);
+  float s = __builtin_amdgcn_exp2f((d.tail - ref) * c);
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += __builtin_amdgcn_exp2f((d.v[j][e] - ref) * c);
+  sum = wave_sum((double)s);
+  // A NaN is no maximum but must not be lost.
+  if (m == -INFINITY && sum != sum) m = -FLT_MAX;
+  m = fminf(m, FLT_MAX);
+}
+
+// The k best classes of a row and the log-sum-exp of the others, one row a
+// workgroup, the row read once (parts of longer rows a second time).
+//
+// Every group of NT / 256 threads has its best (logit, first pack that holds
+// it).  The k-th best of the 256 groups bounds the k-th best class from below,
+// and only about k groups hold classes above the bound: those go to a list in
+// LDS, out of the registers, and each finds its rank by counting the better
+// ones.  What is left in the registers and the list's tail is the rest.  The
+// bound is found by bisection over the groups' order keys, every wave for
+// itself.  A list that overflows (rows whose best classes crowd in few threads)
+// sends the row to k searches for the next best class.
+constexpr int kGroups = 256, kList = 512;
+
+struct TopShared {
+  uint32_t group_key[kGroups], group_pack[kGroups];
+  uint64_t list[kList], sorted[kList];
+  uint64_t red[16];
+  double wave_sum[16];
+  float wave_max[16];
+  int n_list;
+};
+
+// Bound of the list: the composite (key, pack) that at least k groups reach,
+// and few more.
+__device__ __forceinline__ uint64_t top_bound(const TopShared& sh, int k) {
+  const int lane = threadIdx.x & 63;
+  uint32_t key[4], pack[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) key[i] = sh.group_key[i * 64 + lane], pack[i] = sh.group_pack[i * 64 + lane];
+  const auto reach = [&](uint32_t t) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= t));
+    return n;
+  };
+  const uint32_t none = (uint32_t)(kNoKey >> 32);
+  if (reach(none + 1) <= k) return (uint64_t)(none + 1) << 32;
+  uint32_t lo = none + 1;
+  uint32_t hi = wave_max(max(max(key[0], key[1]), max(key[2], key[3]))) + 1;
+  // A smaller start for rows without -inf groups.
+  const uint32_t low = ~wave_max(~min(min(key[0], key[1]), min(key[2], key[3])));
+  lo = max(lo, low);
+  int n = kGroups;
+  const int enough = k + k / 2 + 8;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int c = reach(mid);
+    if (c >= k) {
+      lo = mid;
+      n = c;
+      if (n <= enough) break;
+    } else {
+      hi = mid;
+    }
+  }
+  if (n <= enough) return (uint64_t)lo << 32;
+  // Many groups tie at the bound: the first packs among them.
+  const int need = k - reach(lo + 1);
+  uint32_t plo = 0, phi = 0xFFFFFFFFu;
+  while (phi - plo > 1) {
+    const uint32_t mid = plo + (phi - plo) / 2;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c += __popcll(__ballot(key[i] == lo && pack[i] >= mid));
+    if (c >= need)
+      plo = mid;
+    else
+      phi = mid;
+  }
+  return (uint64_t)lo << 32 | plo;
+}
+
+// The slow way for any row: k searches for the best class below the last one,
+// then the sums of the others, the row read each time.
+template <typename T, bool RULES>
+__device__ __forceinline__ void search_row(const T* x, const RowRules& r, int classes, const TopParams& p, float c,
+                                        int* counts, TopShared& sh, float& wm, double& ws) {
+  const auto each = [&](auto&& f) {
+    for (int first = 0; first < classes; first += kWindow) {
+      const int n = min(kWindow, classes - first);
+      bool counted = false;
+      if constexpr (RULES) {
+        counted = r.n_history > 0;
+        if (counted) {
+          __syncthreads();
+          count_history(r, first, n, counts);
+        }
+      }
+      for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        float v = ld1<T>(x + first + i);
+        if constexpr (RULES) v = apply_rules(r, v, first + i, counted ? counts[i] : 0);
+        f(v, order_key(v, first + i, p.last_ties));
+      }
+    }
+  };
+  uint64_t last = ~0ull;
+  for (int j = 0; j < p.k; ++j) {
+    uint64_t next = 0;
+    each([&](float, uint64_t key) { next = key < last ? max(next, key) : next; });
+    last = block_max(next, sh.red);
+    if (threadIdx.x == 0) sh.sorted[j] = last;
+  }
+  float m = -FLT_MAX;
+  bool some = false;
+  each([&](float v, uint64_t key) {
+    if (key < last && v != -INFINITY) some = true, m = fmaxf(m, v);
+  });
+  m = fminf(wave_max(m), FLT_MAX);
+  double sum = 0.0;
+  each([&](float v, uint64_t key) {
+    if (key < last) sum += (double)__builtin_amdgcn_exp2f((v - m) * c);
+  });
+  wm = __any(some) ? m : -INFINITY;
+  ws = wave_sum(sum);
+}
+
+template <typename T, int NT, int PER, bool RULES>
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : PER * Pack<T>::N <= 32 ? 5 : RULES ? 3 : 4) void top_logits_kernel(LogitRows in, TopParams p, int segs) {
+  constexpr int N = Pack<T>::N, W = NT / 64;
+  __shared__ TopShared sh;
   extern __shared__ int counts[];
-  __shared__ uint64_t red64[16];
-  __shared__ double redd[16];
-  __shared__ float redf[16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(in.x) + row * in.stride;
-  const RowRules r = row_rules(p.rules, row, in.classes);
-  constexpr int kSeg = 8192;
-  uint64_t last = ~0ull;
-  uint64_t found[kMaxTop];
-  for (int j = 0; j < p.k; ++j) {
-    uint64_t best = 0;
-    for (int first = 0; first < in.classes; first += kSeg) {
-      const int n = min(kSeg, in.classes - first);
-      if (r.n_history) count_history(r, first, n, counts);
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = apply_rules(r, ld1<T>(x + first + i), first + i, r.n_history ? counts[i] : 0);
-        const uint64_t key = order_key(v, first + i, p.last_ties);
-        if (key < last) best = max(best, key);
-      }
-      __syncthreads();
-    }
-    last = block_max(best, red64);
-    found[j] = last;
-    if (threadIdx.x == 0 && p.values) {
-      p.values[row * p.k + j] = last > kNoKey ? key_value(last) : -INFINITY;
-      p.indices[row * p.k + j] = last > kNoKey ? key_class(last, p.last_ties) : -1;
-    }
-  }
-  // Log-sum-exp of the others, relative to their own maximum.
+  RowRules r{};
+  if constexpr (RULES) r = row_rules(p.rules, row, in.classes);
+  const int tail_class = in.classes / N * N + tid;
   const float c = kLog2e / p.temperature;
-  float m = -FLT_MAX;
-  double sum = 0.0;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int first = 0; first < in.classes; first += kSeg) {
-      const int n = min(kSeg, in.classes - first);
-      if (r.n_history) count_history(r, first, n, counts);
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = apply_rules(r, ld1<T>(x + first + i), first + i, r.n_history ? counts[i] : 0);
-        if (order_key(v, first + i, p.last_ties) >= last) continue;
-        if (pass == 0)
-          m = fmaxf(m, v);
-        else
-          sum += (double)__builtin_amdgcn_exp2f((v - m) * c);
-      }
-      __syncthreads();
+  if (tid == 0) sh.n_list = 0;
+
+  // Best logit of this thread and the first pack that holds it.
+  RowPart<T, NT, PER> d;
+  float best = -INFINITY;
+  int pack = 0;
+  bool nan = false;
+  int nan_pack = 0;
+  for (int seg = 0; seg < segs; ++seg) {
+    read_part<T, NT, PER, RULES>(d, x, r, in.classes, seg, counts);
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const float m = pack_max(d.v[j]);
+      const bool better = m > best || (p.last_ties && m == best);
+      best = better ? m : best;
+      pack = better ? ((seg * PER + j) * NT + tid) * N : pack;
+#pragma unroll
+      for (int e = 0; e < N; e += 2) bad |= __builtin_isunordered(d.v[j][e], d.v[j][e + 1]);
     }
-    if (pass == 0) m = fminf(block_max(m, redf), FLT_MAX);
+    if (bad && (!nan || p.last_ties)) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (d.v[j][e] != d.v[j][e] && (!nan || p.last_ties)) nan = true, nan_pack = ((seg * PER + j) * NT + tid) * N;
+    }
+    if (seg == 0) {
+      // The single class at the row's end comes after the thread's packs.
+      if (d.tail > best || (p.last_ties && d.tail == best)) best = d.tail, pack = tail_class;
+      if (d.tail != d.tail && (!nan || p.last_ties)) nan = true, nan_pack = tail_class;
+    }
   }
-  sum = block_sum(sum, redd);
-  if (threadIdx.x != 0) return;
-  const double rest = sum > 0.0 || sum != sum ? log(sum) + (double)m / p.temperature : -INFINITY;
-  if (p.rest) p.rest[row] = (float)rest;
+  uint64_t mine = order_key(nan ? NAN : best, nan ? nan_pack : pack, p.last_ties);
+  if constexpr (NT > kGroups) {
+#pragma unroll
+    for (int o = 1; o < NT / kGroups; o <<= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
+  }
+  if (tid % (NT / kGroups) == 0) {
+    sh.group_key[tid / (NT / kGroups)] = (uint32_t)(mine >> 32);
+    sh.group_pack[tid / (NT / kGroups)] = (uint32_t)mine;
+  }
+  __syncthreads();
+
+  // Classes above the bound into the list; the others' sums.
+  const uint64_t bound = top_bound(sh, p.k);
+  const float floor_value = key_value(bound);
+  float wm = -INFINITY;
+  double ws = 0.0;
+  for (int seg = segs - 1; seg >= 0; --seg) {
+    if (seg != segs - 1) read_part<T, NT, PER, RULES>(d, x, r, in.classes, seg, counts);
+    const auto take = [&](float& v, int cls, int at) {
+      const uint64_t key = order_key(v, at, p.last_ties);
+      if (key < bound || key <= kNoKey) return;
+      const int slot = atomicAdd(&sh.n_list, 1);
+      if (slot < kList) sh.list[slot] = order_key(v, cls, p.last_ties);
+      v = -INFINITY;
+    };
+    if (best >= floor_value || nan) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (pack_max(d.v[j]) >= floor_value || nan) {
+          const int at = ((seg * PER + j) * NT + tid) * N;
+#pragma unroll
+          for (int e = 0; e < N; ++e) take(d.v[j][e], at + e, at);
+        }
+      }
+      if (seg == 0) take(d.tail, tail_class, tail_class);
+    }
+    float m;
+    double s;
+    part_sum(d, c, m, s);
+    join_sums(wm, ws, m, s, c);
+  }
+  if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws;
+  __syncthreads();
+
+  int n = sh.n_list;
+  if (n <= kList) {
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t key = sh.list[i];
+      int rank = 0;
+      for (int o = 0; o < n; ++o) rank += sh.list[o] > key;
+      sh.sorted[rank] = key;
+    }
+  } else {
+    search_row<T, RULES>(x, r, in.classes, p, c, counts, sh, wm, ws);
+    n = p.k;
+    if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+
+  // The best of the list, and the rest: the list's tail and the waves' sums.
+  const uint64_t key = lane < min(n, p.k) ? sh.sorted[lane] : 0;
+  const bool any = key > kNoKey;
+  if (p.values && lane < p.k) {
+    p.values[row * p.k + lane] = any ? key_value(key) : -INFINITY;
+    p.indices[row * p.k + lane] = any ? key_class(key, p.last_ties) : -1;
+  }
+  if (!p.rest && !p.pairs) return;
+  float m = lane < W ? sh.wave_max[lane] : -INFINITY;
+  for (int i = p.k + lane; i < n; i += 64) {
+    const float v = key_value(sh.sorted[i]);
+    m = fmaxf(m, v != v ? FLT_MAX : v);
+  }
+  m = fminf(wave_max(m), FLT_MAX);
+  const double inv = 1.0 / (double)p.temperature;
+  double sum = 0.0;
+  if (lane < W && sh.wave_max[lane] > -INFINITY) sum = sh.wave_sum[lane] * exp(((double)sh.wave_max[lane] - m) * inv);
+  for (int i = p.k + lane; i < n; i += 64) sum += exp(((double)key_value(sh.sorted[i]) - m) * inv);
+  sum = wave_sum(sum);
+  const double rest = m == -INFINITY ? -INFINITY : log(sum) + (double)m * inv;
+  if (p.rest && lane == 0) p.rest[row] = (float)rest;
   if (p.pairs) {
-    double top = 0.0;
-    const float v0 = key_value(found[0]);
-    for (int j = 0; j < p.k; ++j)
-      if (found[j] > kNoKey) top += exp(((double)key_value(found[j]) - v0) / p.temperature);
-    const double whole = top + exp(rest - (double)v0 / p.temperature);
-    for (int j = 0; j < p.k; ++j) {
-      const bool any = found[j] > kNoKey;
-      p.pairs[(row * p.k + j) * 2] = any ? (float)key_class(found[j], p.last_ties) : -1.0f;
-      p.pairs[(row * p.k + j) * 2 + 1] =
-          any ? (float)(exp(((double)key_value(found[j]) - v0) / p.temperature) / whole) : 0.0f;
+    const double top = __shfl((double)key_value(key), 0) * inv;
+    const double e = any ? exp((double)key_value(key) * inv - top) : 0.0;
+    const double whole = wave_sum(e) + (m == -INFINITY ? 0.0 : exp(rest - top));
+    if (lane < p.k) {
+      p.pairs[(row * p.k + lane) * 2] = any ? (float)key_class(key, p.last_ties) : -1.0f;
+      p.pairs[(row * p.k + lane) * 2 + 1] = any ? (float)(e / whole) : 0.0f;
     }
   }
 }
@@ -324,15 +657,6 @@ struct TeacherRow {
   double logq;
   double q0, logq0;  // the rest's
 };
-
-__device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
 
 __device__ __forceinline__ TeacherRow teacher_row(const DistillParams& p, int64_t row, int classes) {
   const int lane = threadIdx.x & 63;
@@ -489,13 +813,33 @@ void launch_logit_rules(const LogitRows& in, const RuleParams& rules, void* out,
 #undef RULES_LAUNCH
 }
 
-void launch_top_logits(const LogitRows& in, const TopParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)in.rows);
-  const size_t lds = p.rules.history ? (size_t)std::min(in.classes, 8192) * sizeof(int) : 0;
-  if (in.dt == DT_BF16)
-    hipLaunchKernelGGL(top_logits_kernel<bf16>, grid, dim3(kThreads), lds, s, in, p);
+template <typename T, int NT, int PER, bool RULES>
+void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
+  const int segs = (in.classes + RowPart<T, NT, PER>::kClasses - 1) / RowPart<T, NT, PER>::kClasses;
+  const size_t lds = p.rules.history ? kWindow * sizeof(int) : 0;
+  hipLaunchKernelGGL((top_logits_kernel<T, NT, PER, RULES>), dim3((unsigned)in.rows), dim3(NT), lds, s, in, p, segs);
+}
+
+// Threads of a row's workgroup and the elements that each holds.
+template <typename T, bool RULES>
+void launch_top_typed(const LogitRows& in, const TopParams& p, hipStream_t s) {
+  constexpr int N = Pack<T>::N, kLong = RULES ? 64 : 80;
+  if (in.rows < 512 && in.classes > 256 * 8)
+    in.classes <= 1024 * 32 ? launch_top<T, 1024, 32 / N, RULES>(in, p, s)
+                            : launch_top<T, 1024, kLong / N, RULES>(in, p, s);
+  else if (in.classes <= 256 * 32)
+    launch_top<T, 256, 32 / N, RULES>(in, p, s);
+  else if (in.classes <= 256 * 80)
+    launch_top<T, 256, 80 / N, RULES>(in, p, s);
   else
-    hipLaunchKernelGGL(top_logits_kernel<float>, grid, dim3(kThreads), lds, s, in, p);
+    launch_top<T, 1024, kLong / N, RULES>(in, p, s);
+}
+
+void launch_top_logits(const LogitRows& in, const TopParams& p, hipStream_t s) {
+  if (p.rules.history || p.rules.bias || p.rules.masks)
+    in.dt == DT_BF16 ? launch_top_typed<bf16, true>(in, p, s) : launch_top_typed<float, true>(in, p, s);
+  else
+    in.dt == DT_BF16 ? launch_top_typed<bf16, false>(in, p, s) : launch_top_typed<float, false>(in, p, s);
 }
 
 void launch_distill(const LogitRows& student, const DistillParams& p, hipStream_t s) {

@@ -219,6 +219,56 @@ def test_top_of_ties_and_orders(gpu, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,classes", [(2, 9000), (600, 8000), (2, 40000)])
+def test_top_of_crowded_threads(gpu, rows, classes, dtype):
+    """All large logits at places that few threads of a workgroup hold, so that
+    far more classes than k lie above the bound that the threads' best give."""
+    rng = np.random.default_rng(classes)
+    pack = 4 if dtype == "f32" else 8
+    for period, width in ((256 * pack, pack), (1024 * pack, 4 * pack)):
+        group = np.arange(classes) % period // width
+        x = np.where(group < 63, 10 + rng.random(classes), np.where(group == 63, 5.0, -np.arange(classes) / classes))
+        x = torch.from_numpy(x.astype(np.float32)).to(TYPE[dtype]).cuda().repeat(rows, 1)
+        kw = make_rules(rng, 1, classes, ("bias", "history"))
+        kw = dict(bias=kw["bias"][:1] * 0.01, history=np.arange(50, dtype=np.int32),
+                  history_offsets=np.append(0, np.full(rows, 50)), presence=np.full(rows, 0.01, np.float32))
+        for rules in (None, kw):
+            # The history is the first row's; all others are alike.
+            y = f32(x[:2])
+            if rules is not None:
+                y = oracle.rules(y, kw["bias"], history=kw["history"], history_offsets=[0, 50, 50],
+                                 presence=kw["presence"][:2])
+            values, indices, rest, error = (np.concatenate([a[:1], np.repeat(a[1:], rows - 1, 0)])
+                                            for a in oracle.top(y, 64, 1.0))
+            got = gpu.top_logits(x, 64, None if rules is None else on_device(classes, rules))
+            assert np.array_equal(f32(got.values), values) and np.array_equal(got.indices.cpu().numpy(), indices)
+            assert np.all(np.abs(f32(got.rest) - rest) <= error)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [300, 6906, 18710, 30000])
+def test_top_of_many_rows(gpu, classes, dtype):
+    """Batches take other workgroups than a few rows do: the rows of a batch
+    against the plain form, under rules and without."""
+    rng = np.random.default_rng(classes)
+    x = rows_of(rng, 24, classes, dtype, 1)
+    kw = make_rules(rng, 24, classes, ("bias", "mask", "history"))
+    many = x.repeat(25, 1)
+    lengths = np.diff(kw["history_offsets"])
+    big = {k: np.tile(v, 25) for k, v in kw.items() if k in ("row_bias", "row_mask", "repetition", "frequency", "presence", "history")}
+    big.update(bias=kw["bias"], masks=kw["masks"], history_offsets=np.append(0, np.cumsum(np.tile(lengths, 25))))
+    for k in (1, 30, 64):
+        for rules, y in ((None, f32(x)), (on_device(classes, big), oracle.rules(f32(x), **kw))):
+            values, indices, rest, error = oracle.top(y, k, 1.0)
+            got = gpu.top_logits(many, k, rules)
+            assert np.array_equal(f32(got.values).reshape(25, 24, k), np.broadcast_to(values, (25, 24, k)))
+            assert np.array_equal(got.indices.cpu().numpy().reshape(25, 24, k), np.broadcast_to(indices, (25, 24, k)))
+            g = f32(got.rest).astype(np.float64).reshape(25, 24)
+            with np.errstate(invalid="ignore"):
+                assert np.all((np.abs(g - rest) <= error) | (g == rest))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_top_of_rows_with_few_candidates(gpu, dtype):
     x = torch.full((6, 500), -INF, device="cuda")
     x[1, 499] = 2.0
