@@ -234,15 +234,6 @@ __device__ __forceinline__ V block_max(V v, V* red) {
   for (int i = 1; i < (int)(blockDim.x >> 6); ++i) r = max(r, red[i]);
   return r;
 }
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double r = red[0];
-  for (int i = 1; i < (int)(blockDim.x >> 6); ++i) r += red[i];
-  return r;
-}
 __device__ __forceinline__ double wave_sum(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
@@ -648,145 +639,238 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : PER * Pack<T>::N <= 32 ? 5 : R
   }
 }
 
-// The teacher's shares of one row, by one wave (k <= 64: one entry a lane).
-struct TeacherRow {
-  bool valid;    // this lane's entry counts
-  bool any;      // some lane's does
-  int index;     // its class
-  double q;      // its share
-  double logq;
-  double q0, logq0;  // the rest's
+// An entry of a teacher's row, one a lane (k <= 64).
+struct TeacherEntry {
+  int index;  // its class, -1: does not count (a class named twice is not looked for yet)
+  float value;
 };
-
-__device__ __forceinline__ TeacherRow teacher_row(const DistillParams& p, int64_t row, int classes) {
+__device__ __forceinline__ TeacherEntry teacher_entry(const DistillParams& p, int64_t row, int classes) {
   const int lane = threadIdx.x & 63;
-  TeacherRow t;
-  t.index = -1;
-  float v = -INFINITY;
+  TeacherEntry t{-1, -INFINITY};
   if (lane < p.k) {
     t.index = p.indices[row * p.k + lane];
-    v = p.values[row * p.k + lane];
+    t.value = p.values[row * p.k + lane];
   }
-  t.valid = t.index >= 0 && t.index < classes && v != -INFINITY;
-  if (!t.valid) t.index = -1;
-  // A class named twice counts once, with its first entry.
-  for (int j = 0; j < p.k; ++j) {
-    const int other = __shfl(t.index, j);
-    if (j < lane && other == t.index) t.valid = false;
-  }
-  t.any = __any(t.valid);
-  if (!t.any) return t;
-  const double inv = 1.0 / (double)p.temperature;
-  const double d = t.valid ? (double)v * inv : -INFINITY;
-  const double rest = p.rest ? (double)p.rest[row] : -INFINITY;
-  const double m = fmax((double)wave_max(t.valid ? v : -INFINITY) * inv, rest);
-  const double sum = wave_sum(t.valid ? exp(d - m) : 0.0) + exp(rest - m);
-  const double logsum = log(sum);
-  t.logq = d - m - logsum;
-  t.q = t.valid ? exp(t.logq) : 0.0;
-  t.logq0 = rest - m - logsum;
-  t.q0 = exp(t.logq0);
+  if (t.index < 0 || t.index >= classes || t.value == -INFINITY) t.index = -1;
   return t;
 }
 
-// Gradient of the row from its sums: classes of the rest, then the entries.
-template <typename T>
-__device__ __forceinline__ void distill_row_grad(const LogitRows& s, const DistillParams& p, int64_t row, float m,
-                                                 float z, float mr, float zr, const TeacherRow& t, float entry) {
+// The teacher's shares of a row, by one wave, in 64 bits: the loss is a
+// difference of logs that nearly cancel.
+struct TeacherShares {
+  bool valid;     // this lane's entry counts
+  double q, logq;  // its share
+  double q0, logq0;  // the rest's
+};
+__device__ __forceinline__ TeacherShares teacher_shares(const DistillParams& p, int64_t row, const TeacherEntry& e,
+                                                        double inv) {
+  const int lane = threadIdx.x & 63;
+  TeacherShares t;
+  t.valid = e.index >= 0;
+  // A class named twice counts once, with its first entry.
+  for (int j = 0; j + 1 < p.k; ++j)
+    if (__builtin_amdgcn_readlane(e.index, j) == e.index && j < lane) t.valid = false;
+  const double rest = p.rest ? (double)p.rest[row] : -INFINITY;
+  const double m = fmax((double)wave_max(t.valid ? e.value : -INFINITY) * inv, rest);
+  const double d = (double)e.value * inv - m;
+  const double x = t.valid ? exp(d) : 0.0, x0 = exp(rest - m);
+  const double sum = wave_sum(x) + x0, logsum = log(sum);
+  t.q = x / sum;
+  t.logq = d - logsum;
+  t.q0 = x0 / sum;
+  t.logq0 = rest - m - logsum;
+  return t;
+}
+
+// Distillation of one row a workgroup: its loss, its gradient, or both.
+//
+// With e_c = exp((s_c - M) / tau), Z0 the sum of e over the classes that are no
+// entry, Z = Z0 + sum over the entries, p = e / Z and the rest's share of the
+// student p0 = Z0 / Z:
+//   loss = tau^2 (sum_j q_j (log q_j - log p_j) + q0 (log q0 - log p0)),
+//   d loss / d s_c = tau (p_c - q_c) for an entry, tau e_c (1 / Z - q0 / Z0) else.
+// So the rest's gradient is e times one factor of the row, and the row is read
+// once: it stays in registers with the entries taken out (their marks come
+// through LDS, a byte a pack), first as logits, then as exponentials relative
+// to the wave's maximum.  Wave 0 does the entries, in 64 bits, while the others
+// sum, and writes their gradients over the row's.  The whole is formed from the
+// rest and the entries, so that the shares add up to one and an error of the
+// rest's sum cancels to first order in the loss.  Rows longer than the
+// registers go through them in parts, twice when the gradient is asked for.
+enum DistillMode { kLoss, kBoth, kGradient };
+
+struct DistillShared {
+  double sum[16];
+  float max[16];
+  float factor[16];
+  float top;  // maximum of the rest
+};
+
+// PARTS: rows of `segs` parts; else the whole row is one.
+template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : PER * Pack<T>::N <= 32 ? 6 : 4) void distill_kernel(
+    LogitRows s, DistillParams p, int parts) {
+  constexpr int N = Pack<T>::N, W = NT / 64, kWords = (PER + 3) / 4;
+  __shared__ DistillShared sh;
+  __shared__ uint32_t marks[MODE == kGradient ? 1 : NT * kWords];
+  const int segs = PARTS ? parts : 1;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const int full = s.classes / N, tail_class = full * N + tid;
+  const bool has_tail = tail_class < s.classes;
   const T* x = static_cast<const T*>(s.x) + row * s.stride;
   T* g = static_cast<T*>(p.grad) + row * p.grad_stride;
-  const float scale = (p.grad_loss ? p.grad_loss[row] : 1.0f) * p.temperature;
-  const float c = kLog2e / p.temperature;
-  const bool dead = m == -INFINITY;
-  const float share = zr > 0.0f ? (float)(t.q0 * exp(((double)m - mr) / p.temperature) * z / zr) : 0.0f;
-  const float k = dead ? 0.0f : scale * (1.0f - share) / z;
-  for (int i = threadIdx.x; i < s.classes; i += kThreads) {
-    const float v = ld1<T>(x + i);
-    st1<T>(g + i, dead ? 0.0f : k * __builtin_amdgcn_exp2f((v - m) * c));
-  }
-  __syncthreads();
-  if (threadIdx.x < 64 && t.valid)
-    st1<T>(g + t.index, dead ? 0.0f : scale * (__builtin_amdgcn_exp2f((entry - m) * c) / z - (float)t.q));
-}
-
-template <typename T>
-__device__ __forceinline__ void zero_row(T* g, int n) {
-  for (int i = threadIdx.x; i < n; i += kThreads) st1<T>(g + i, 0.0f);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_kernel(LogitRows s, DistillParams p) {
-  extern __shared__ uint32_t bits[];
-  __shared__ double redd[16];
-  __shared__ float redf[16];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(s.x) + row * s.stride;
-  const TeacherRow t = teacher_row(p, row, s.classes);
-  if (!t.any) {
-    if (threadIdx.x == 0) {
-      if (p.loss) p.loss[row] = 0.0f;
-      if (p.state)
-        for (int i = 0; i < 4; ++i) p.state[row * 4 + i] = 0.0f;
+  const TeacherEntry entry = teacher_entry(p, row, s.classes);
+  if (!__any(entry.index >= 0)) {
+    if (MODE != kGradient && tid == 0) p.loss[row] = 0.0f;
+    if (MODE == kLoss && p.state && tid < 4) p.state[row * 4 + tid] = 0.0f;
+    if (MODE != kLoss) {
+      const float zero[N] = {};
+      for (int i = tid; i < full; i += NT) Pack<T>::store(g + i * N, zero);
+      if (has_tail) st1<T>(g + tail_class, 0.0f);
     }
-    if (p.grad) zero_row<T>(static_cast<T*>(p.grad) + row * p.grad_stride, s.classes);
     return;
   }
-  const int words = (s.classes + 31) / 32;
-  for (int i = threadIdx.x; i < words; i += kThreads) bits[i] = 0;
-  __syncthreads();
-  float entry = 0.0f;
-  if (threadIdx.x < 64 && t.valid) {
-    atomicOr(&bits[t.index >> 5], 1u << (t.index & 31));
-    entry = ld1<T>(x + t.index);
-  }
-  __syncthreads();
   const float c = kLog2e / p.temperature;
   const double inv = 1.0 / (double)p.temperature;
-  float mr = -INFINITY;
-  for (int i = threadIdx.x; i < s.classes; i += kThreads)
-    if (!(bits[i >> 5] >> (i & 31) & 1)) mr = fmaxf(mr, ld1<T>(x + i));
-  mr = block_max(mr, redf);
-  const float low = fmaxf(mr, -FLT_MAX);
+  // The entries' own logits, before a gradient in place covers them.
+  float own = 0.0f;
+  if (wave == 0 && entry.index >= 0) own = ld1<T>(x + entry.index);
+
+  RowPart<T, NT, PER> d;
+  float m = -INFINITY;  // the wave's maximum and sum of the rest
   double sum = 0.0;
-  for (int i = threadIdx.x; i < s.classes; i += kThreads)
-    if (!(bits[i >> 5] >> (i & 31) & 1)) sum += (double)__builtin_amdgcn_exp2f((ld1<T>(x + i) - low) * c);
-  const double zr = block_sum(sum, redd);
-  const float m = block_max(threadIdx.x < 64 && t.valid ? fmaxf(entry, mr) : mr, redf);
-  const float mlow = fmaxf(m, -FLT_MAX);
-  // The whole is the entries and the rest: shares add up to one, and an error
-  // of the rest's sum cancels to first order in the loss.
-  const double e = threadIdx.x < 64 && t.valid ? exp(((double)entry - mlow) * inv) : 0.0;
-  const double z = block_sum(e, redd) + zr * exp(((double)low - mlow) * inv);
-  double term = 0.0;
-  const double logz = log(z);
-  if (threadIdx.x < 64 && t.valid && t.q > 0.0) term = t.q * (t.logq - (((double)entry - mlow) * inv - logz));
-  if (threadIdx.x == 0 && t.q0 > 0.0) term += t.q0 * (t.logq0 - (((double)low - mlow) * inv + log(zr) - logz));
-  const double loss = block_sum(term, redd) * (double)p.temperature * (double)p.temperature;
-  if (threadIdx.x == 0) {
-    if (p.loss) p.loss[row] = m == -INFINITY ? INFINITY : (float)loss;
-    if (p.state) {
-      p.state[row * 4 + 0] = m;
-      p.state[row * 4 + 1] = (float)z;
-      p.state[row * 4 + 2] = mr;
-      p.state[row * 4 + 3] = (float)zr;
+  if constexpr (MODE != kGradient) {
+    for (int seg = 0; seg < segs; ++seg) {
+      load_part(d, x, s.classes, seg);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) marks[tid * kWords + i] = 0;
+      __syncthreads();
+      if (wave == 0 && entry.index >= 0) {
+        const int i = entry.index / N, at = i - seg * PER * NT;
+        if (i < full && at >= 0 && at < PER * NT) {
+          const int j = at / NT;
+          atomicOr(&marks[(at - j * NT) * kWords + (j >> 2)], 1u << ((j & 3) * 8 + entry.index % N));
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const uint32_t word = marks[tid * kWords + w];
+        if (word)
+#pragma unroll
+          for (int q = 0; q < 4 && w * 4 + q < PER; ++q)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (word >> (q * 8 + e) & 1) d.v[w * 4 + q][e] = -INFINITY;
+      }
+      if (seg == 0 && __any(entry.index >= full * N)) {
+        // Entries among the row's last classes, one a thread.
+        for (int j = 0; j < p.k; ++j)
+          if (__builtin_amdgcn_readlane(entry.index, j) == tail_class) d.tail = -INFINITY;
+      }
+      float t = d.tail;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) t = fmaxf(t, pack_max(d.v[j]));
+      t = wave_max(t);
+      const float ref = fmaxf(t, -FLT_MAX);
+      d.tail = __builtin_amdgcn_exp2f((d.tail - ref) * c);
+      float part = d.tail;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          d.v[j][e] = __builtin_amdgcn_exp2f((d.v[j][e] - ref) * c);
+          part += d.v[j][e];
+        }
+      const double ps = wave_sum((double)part);
+      if (ps != ps) t = ref;  // a NaN is no maximum but must not be lost
+      join_sums(m, sum, t, ps, c);
+      if (PARTS) __syncthreads();  // the marks are no longer read
+    }
+    if (lane == 0) sh.max[wave] = m, sh.sum[wave] = sum;
+    __syncthreads();
+  } else if (!PARTS) {
+    load_part(d, x, s.classes, 0);
+  }
+
+  float entry_grad = 0.0f;
+  bool entry_valid = false;
+  if (wave == 0) {
+    const TeacherShares t = teacher_shares(p, row, entry, inv);
+    entry_valid = t.valid;
+    double top, z, mr, zr;
+    if constexpr (MODE == kGradient) {
+      const float* st = p.state + row * 4;
+      top = st[0], z = st[1], mr = st[2], zr = st[3];
+    } else {
+      const float om = lane < W ? sh.max[lane] : -INFINITY;
+      const float rm = wave_max(om);
+      // Sums of the waves; a wave without any class of the rest has none.
+      zr = wave_sum(om > -INFINITY ? sh.sum[lane] * exp(((double)om - rm) * inv) : 0.0);
+      mr = rm;
+      const float em = fmaxf(rm, wave_max(t.valid ? own : -INFINITY));
+      top = em;
+    }
+    const double low = fmax(top, -(double)FLT_MAX);
+    const double a = ((double)own - low) * inv;
+    const double e = t.valid ? exp(a) : 0.0;
+    const double e0 = mr == -INFINITY ? 0.0 : exp((mr - low) * inv);  // of the rest's maximum
+    if constexpr (MODE != kGradient) {
+      z = wave_sum(e) + zr * e0;
+      const double logz = log(z);
+      double term = t.valid && t.q > 0.0 ? t.q * (t.logq - (a - logz)) : 0.0;
+      if (lane == 0 && t.q0 > 0.0) term += t.q0 * (t.logq0 - (zr > 0.0 || zr != zr ? (mr - low) * inv + log(zr) - logz : -INFINITY));
+      const double loss = wave_sum(term) * (double)p.temperature * (double)p.temperature;
+      if (lane == 0) {
+        p.loss[row] = top == -INFINITY && !(z != z) ? INFINITY : (float)loss;
+        if (MODE == kLoss && p.state) {
+          p.state[row * 4 + 0] = (float)top;
+          p.state[row * 4 + 1] = (float)z;
+          p.state[row * 4 + 2] = (float)mr;
+          p.state[row * 4 + 3] = (float)zr;
+        }
+      }
+    }
+    if constexpr (MODE != kLoss) {
+      const double scale = (p.grad_loss ? (double)p.grad_loss[row] : 1.0) * (double)p.temperature;
+      // No class has any probability: no gradient.
+      const bool dead = top == -INFINITY && !(z != z);
+      // Of exponentials relative to the rest's maximum: its classes may be far
+      // below the entries and still share q0 among them.
+      const double factor = dead || zr == 0.0 ? 0.0 : scale * (e0 / z - t.q0 / zr);
+      entry_grad = dead ? 0.0f : (float)(scale * (e / z - t.q));
+      if (MODE == kBoth && !PARTS) {
+        // The registers hold exponentials of each wave's own maximum.
+        if (lane < W) sh.factor[lane] = sh.max[lane] == -INFINITY ? 0.0f : (float)(factor * exp(((double)sh.max[lane] - mr) * inv));
+      } else if (lane == 0) {
+        sh.factor[0] = (float)factor;
+        sh.top = (float)fmax(mr, -(double)FLT_MAX);
+      }
     }
   }
-  if (p.grad) distill_row_grad<T>(s, p, row, m, (float)z, mr, (float)zr, t, entry);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_grad_kernel(LogitRows s, DistillParams p) {
-  const int64_t row = blockIdx.x;
-  const TeacherRow t = teacher_row(p, row, s.classes);
-  if (!t.any) {
-    zero_row<T>(static_cast<T*>(p.grad) + row * p.grad_stride, s.classes);
-    return;
+  if constexpr (MODE != kLoss) {
+    __syncthreads();
+    constexpr bool kReady = MODE == kBoth && !PARTS;
+    const float factor = sh.factor[kReady ? wave : 0], ref = kReady ? 0.0f : sh.top;
+    for (int seg = segs - 1; seg >= 0; --seg) {
+      if (PARTS) load_part(d, x, s.classes, seg);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = (seg * PER + j) * NT + tid;
+        if (i >= full) continue;
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          v[e] = factor * (kReady ? d.v[j][e] : __builtin_amdgcn_exp2f((d.v[j][e] - ref) * c));
+        Pack<T>::store(g + i * N, v);
+      }
+      if (seg == 0 && has_tail)
+        st1<T>(g + tail_class, factor * (kReady ? d.tail : __builtin_amdgcn_exp2f((d.tail - ref) * c)));
+    }
+    __syncthreads();
+    if (wave == 0 && entry_valid) st1<T>(g + entry.index, entry_grad);
   }
-  float entry = 0.0f;
-  if (threadIdx.x < 64 && t.valid) entry = ld1<T>(static_cast<const T*>(s.x) + row * s.stride + t.index);
-  __syncthreads();
-  const float* st = p.state + row * 4;
-  distill_row_grad<T>(s, p, row, st[0], st[1], st[2], st[3], t, entry);
 }
 
 }  // namespace
@@ -842,21 +926,37 @@ void launch_top_logits(const LogitRows& in, const TopParams& p, hipStream_t s) {
     in.dt == DT_BF16 ? launch_top_typed<bf16, false>(in, p, s) : launch_top_typed<float, false>(in, p, s);
 }
 
-void launch_distill(const LogitRows& student, const DistillParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)student.rows);
-  const size_t lds = (size_t)((student.classes + 31) / 32) * sizeof(uint32_t);
-  if (student.dt == DT_BF16)
-    hipLaunchKernelGGL(distill_kernel<bf16>, grid, dim3(kThreads), lds, s, student, p);
+template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
+void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  const int parts = (in.classes + RowPart<T, NT, PER>::kClasses - 1) / RowPart<T, NT, PER>::kClasses;
+  hipLaunchKernelGGL((distill_kernel<T, NT, PER, PARTS, MODE>), dim3((unsigned)in.rows), dim3(NT), 0, s, in, p, parts);
+}
+
+// Threads of a row's workgroup and the elements that each holds.
+template <typename T, DistillMode MODE>
+void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  constexpr int N = Pack<T>::N;
+  if (in.rows < 512 && in.classes > 256 * 8 && in.classes <= 1024 * 32)
+    launch_distill_one<T, 1024, 32 / N, false, MODE>(in, p, s);
+  else if (in.classes <= 256 * 32)
+    launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
+  else if (in.classes <= 256 * 80)
+    launch_distill_one<T, 256, 80 / N, false, MODE>(in, p, s);
   else
-    hipLaunchKernelGGL(distill_kernel<float>, grid, dim3(kThreads), lds, s, student, p);
+    launch_distill_one<T, 1024, 80 / N, true, MODE>(in, p, s);
+}
+
+template <DistillMode MODE>
+void launch_distill_mode(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  in.dt == DT_BF16 ? launch_distill_typed<bf16, MODE>(in, p, s) : launch_distill_typed<float, MODE>(in, p, s);
+}
+
+void launch_distill(const LogitRows& student, const DistillParams& p, hipStream_t s) {
+  p.grad ? launch_distill_mode<kBoth>(student, p, s) : launch_distill_mode<kLoss>(student, p, s);
 }
 
 void launch_distill_grad(const LogitRows& student, const DistillParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)student.rows);
-  if (student.dt == DT_BF16)
-    hipLaunchKernelGGL(distill_grad_kernel<bf16>, grid, dim3(kThreads), 0, s, student, p);
-  else
-    hipLaunchKernelGGL(distill_grad_kernel<float>, grid, dim3(kThreads), 0, s, student, p);
+  launch_distill_mode<kGradient>(student, p, s);
 }
 
 }  // namespace ppocr

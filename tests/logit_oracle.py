@@ -162,18 +162,17 @@ def distill(x, values, indices, rest, tau, grad_loss=None):
             # The rest's sum enters each log p through the whole, and the rest's once more.
             loss_err[r] = tau * tau * 2 * er + 2 * U * abs(loss[r]) + 1e-12
             p = np.exp((x[r] - m) / tau - logz)
-            p0 = np.exp(logp[-1])
-            share = q[-1] / p0 if q[-1] > 0 and p0 > 0 else 0.0
-            grad[r] = np.where(entry, 0.0, np.where(p > 0, p * (1 - share), 0.0))
+            # The rest's shares of itself: far below the entries they still add up to one.
+            own = np.where(entry | (x[r] == -INF), 0.0, np.exp((x[r] - low) / tau) / zr if zr > 0 else 0.0)
+            grad[r] = np.where(entry, 0.0, p - q[-1] * own)
             grad[r][at] = p[at] - q[:-1]
             grad[r] *= tau * g[r]
-            # p: the exponential's argument and itself, the sums, a division and
-            # the scale; the share: both sums, two exponentials and its products.
+            # The exponential's argument and itself, the sums, a division and the scale.
             d = np.where(p > 0, np.abs(x[r] - m) / tau, 0.0)
-            rel = (3 * d + 8) * U + er
-            part = np.where(entry, 0.0, share)
+            d0 = np.where(own > 0, np.abs(x[r] - low) / tau, 0.0)
             q_of = np.zeros(classes)
             q_of[at] = q[:-1]
-            grad_err[r] = tau * abs(g[r]) * (p * (1 + part) * rel + p * part * (er + 8 * U) + 4 * U * q_of) + 4 * U * np.abs(grad[r])
+            grad_err[r] = tau * abs(g[r]) * (p * ((3 * d + 8) * U + er) + q[-1] * own * ((3 * d0 + 8) * U + er) + 4 * U * q_of)
+            grad_err[r] += 4 * U * np.abs(grad[r])
             grad_err[r] += tau * abs(g[r]) * 1e-37  # exponentials below the normal range may flush
     return loss, state, grad, loss_err, state_err, grad_err

@@ -346,6 +346,29 @@ def test_distill(gpu, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [301, 6907, 18710, 30000])
+def test_distill_of_many_rows(gpu, classes, dtype):
+    """Batches take other workgroups than a few rows do: rows of a batch
+    against the plain form."""
+    rng = np.random.default_rng(classes)
+    x = rows_of(rng, 600, classes, dtype, 1)
+    values, indices, rest = np.zeros((600, 12), np.float32), np.full((600, 12), -1, np.int32), np.zeros(600, np.float32)
+    values[:20], indices[:20], rest[:20] = teacher_of(rng, x[:20], 12, 1.5)
+    g = rng.uniform(0.5, 1.5, 600).astype(np.float32)
+    teacher = ppocr_hip.TopLogits(dev(values), i32(indices), dev(rest))
+    loss, grad = gpu.distill(x, teacher, 1.5, dev(g))
+    only, state = gpu.distill_loss(x, teacher, 1.5)
+    apart = gpu.distill_grad(x, teacher, state, 1.5, dev(g))
+    for got in (loss, grad, only, state, apart):
+        assert (got[20:] == 0).all()  # without a target
+    want_loss, _, want, loss_err, _, err = oracle.distill(f32(x[:20]), values[:20], indices[:20], rest[:20], 1.5, g[:20])
+    err = err + HALF[dtype] * np.abs(want) * (1 + 2.0 ** -7) + 2.0 ** -134
+    assert np.all(np.abs(f32(loss[:20]) - want_loss) <= loss_err) and np.all(np.abs(f32(only[:20]) - want_loss) <= loss_err)
+    assert np.all(np.abs(f32(grad[:20]) - want) <= err)
+    assert np.all(np.abs(f32(apart[:20]) - want) <= err + 8 * oracle.U * np.abs(want) + 4 * oracle.U * 1.5 * g[:20, None] * (want != 0))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("classes", [40, 6906, 18710])
 def test_distill_of_ragged_teachers(gpu, classes, dtype):
     """Rows without a target, classes named twice or outside the row, entries
@@ -384,6 +407,22 @@ def test_distill_of_masked_students(gpu, dtype):
         both = check_distill(gpu, x, values, indices, rest, 1.0, dtype)
         assert (both[2] == 0).all()
         check_distill(gpu, x, values, indices, None, 1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes,low", [(50, -200.0), (50, None), (20001, -200.0), (20001, None), (100003, -90.0)])
+def test_distill_of_a_rest_far_below_the_entries(gpu, classes, low, dtype):
+    """The student gives the rest next to nothing, the teacher a share of it:
+    each class of the rest still draws its part of that share."""
+    rng = np.random.default_rng(13)
+    x = rows_of(rng, 3, classes, dtype)
+    values, indices, rest = teacher_of(rng, x, 6, 1.0)
+    others = torch.ones(3, classes, dtype=torch.bool, device="cuda")
+    others.scatter_(1, torch.from_numpy(indices.astype(np.int64)).cuda(), False)
+    x[others] = LOWEST[dtype] if low is None else low
+    rest = (values.max(1) + 1.0).astype(np.float32)
+    grad = check_distill(gpu, x, values, indices, rest, 1.0, dtype)
+    assert (grad[others] < 0).all()
 
 
 @pytest.mark.parametrize("bad", [float("nan"), INF])
