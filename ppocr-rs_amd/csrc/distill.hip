@@ -1,0 +1,271 @@
+// Distillation of rows of class logits from a teacher's best classes.
+#include "logit_rows.h"
+
+namespace ppocr {
+namespace {
+
+// An entry of a teacher's row, one a lane (k <= 64).
+struct TeacherEntry {
+  int index;  // its class, -1: does not count (a class named twice is not looked for yet)
+  float value;
+};
+__device__ __forceinline__ TeacherEntry teacher_entry(const DistillParams& p, int64_t row, int classes) {
+  const int lane = threadIdx.x & 63;
+  TeacherEntry t{-1, -INFINITY};
+  if (lane < p.k) {
+    t.index = p.indices[row * p.k + lane];
+    t.value = p.values[row * p.k + lane];
+  }
+  if (t.index < 0 || t.index >= classes || t.value == -INFINITY) t.index = -1;
+  return t;
+}
+
+// Distillation of one row a workgroup: its loss, its gradient, or both.
+//
+// With e_c = exp((s_c - M) / tau), Z0 the sum of e over the classes that are no
+// entry, Z = Z0 + sum over the entries, p = e / Z and the rest's share of the
+// student p0 = Z0 / Z:
+//   loss = tau^2 (sum_j q_j (log q_j - log p_j) + q0 (log q0 - log p0)),
+//   d loss / d s_c = tau (p_c - q_c) for an entry, tau e_c (1 / Z - q0 / Z0) else.
+// So the rest's gradient is e times one factor of the row, and the row is read
+// once: it stays in registers with the entries taken out (their marks come
+// through LDS, a byte a pack).  Wave 0 does the entries, in 64 bits, the
+// teacher's shares while the row is on its way, and writes their gradients over
+// the row's.  The whole is formed from the rest and the entries, so that the
+// shares add up to one and an error of the rest's sum cancels to first order in
+// the loss.  Rows longer than the registers go through them in parts, twice when
+// the gradient is asked for.
+enum DistillMode { kLoss, kBoth, kGradient };
+
+struct DistillShared {
+  double sum[16];
+  float max[16];
+  float factor, top;  // of the rest's gradient: exp((s - top) / tau) times factor
+  double q[64], logq[64];  // the teacher's shares, which wave 0 keeps here rather than in registers
+  double q0, logq0;
+};
+
+// Waves a SIMD that the registers of a part leave room for.
+template <typename T, int NT, int PER, bool PARTS>
+constexpr int distill_waves() {
+  constexpr int regs = PER * 4;
+  return NT == 1024 && PARTS ? 4 : regs <= 16 ? 8 : regs <= 40 ? 6 : 4;
+}
+
+// The teacher's shares of a row and their logs, by wave 0, in 64 bits: the loss
+// is a difference of logs that nearly cancel.  An entry that does not count
+// loses its index.
+__device__ __forceinline__ void teacher_shares(const DistillParams& p, int64_t row, TeacherEntry& entry, double inv,
+                                               DistillShared& sh) {
+  const int lane = threadIdx.x & 63;
+  // A class named twice counts once, with its first entry.
+  bool again = false;
+  for (int j = 0; j + 1 < p.k; ++j) again |= __builtin_amdgcn_readlane(entry.index, j) == entry.index && j < lane;
+  if (again) entry.index = -1;
+  const bool valid = entry.index >= 0;
+  const double rest = p.rest ? (double)p.rest[row] : -INFINITY;
+  const double m = fmax((double)wave_max(valid ? entry.value : -INFINITY) * inv, rest);
+  const double d = (double)entry.value * inv - m;
+  const double x = valid ? exp(d) : 0.0, x0 = exp(rest - m);
+  const double sum = wave_sum(x) + x0, logsum = log(sum);
+  sh.q[lane] = x / sum;
+  sh.logq[lane] = d - logsum;
+  if (lane == 0) sh.q0 = x0 / sum, sh.logq0 = rest - m - logsum;
+}
+
+// PARTS: rows of `parts` parts; else the whole row is one.
+template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
+__global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void distill_kernel(LogitRows s, DistillParams p, int parts) {
+  constexpr int N = Pack<T>::N, W = NT / 64, kWords = (PER + 3) / 4;
+  __shared__ DistillShared sh;
+  __shared__ uint32_t marks[MODE == kGradient ? 1 : NT * kWords];
+  const int segs = PARTS ? parts : 1;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const RowShape<N> shape(s.classes, 0);
+  const T* x = static_cast<const T*>(s.x) + row * s.stride;
+  T* g = static_cast<T*>(p.grad) + row * p.grad_stride;
+  TeacherEntry entry = teacher_entry(p, row, s.classes);
+  if (!__any(entry.index >= 0)) {
+    if (MODE != kGradient && tid == 0) p.loss[row] = 0.0f;
+    if (MODE == kLoss && p.state && tid < 4) p.state[row * 4 + tid] = 0.0f;
+    if (MODE != kLoss) {
+      const float zero[N] = {};
+      for (int i = tid; i < shape.full; i += NT) Pack<T>::store(g + i * N, zero);
+      if (shape.has_tail()) st1<T>(g + shape.tail_class(), 0.0f);
+    }
+    return;
+  }
+  const float c = kLog2e / p.temperature;
+  const double inv = 1.0 / (double)p.temperature;
+  // The entries' own logits, before a gradient in place covers them.
+  float own = 0.0f;
+  if (wave == 0 && entry.index >= 0) own = ld1<T>(x + entry.index);
+
+  RowPart<T, NT, PER, true> d;
+  float m = -INFINITY;  // the wave's maximum and sum of the rest
+  double sum = 0.0;
+  if (!PARTS || MODE != kGradient) load_part(d, x, shape, 0);
+  if constexpr (MODE != kGradient) {
+    for (int seg = 0; seg < segs; ++seg) {
+      if (seg > 0) load_part(d, x, shape, seg);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) marks[tid * kWords + i] = 0;
+      __syncthreads();
+      if (wave == 0 && entry.index >= 0) {
+        const int i = entry.index / N, at = i - seg * PER * NT;
+        if (i < shape.full && at >= 0 && at < PER * NT) {
+          const int j = at / NT;
+          atomicOr(&marks[(at - j * NT) * kWords + (j >> 2)], 1u << ((j & 3) * 8 + entry.index % N));
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const uint32_t word = marks[tid * kWords + w];
+        if (word)
+#pragma unroll
+          for (int q = 0; q < 4 && w * 4 + q < PER; ++q)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (word >> (q * 8 + e) & 1) d.pack[w * 4 + q].clear(e);
+      }
+      if (seg == 0 && __any(entry.index >= shape.full * N)) {
+        // Entries among the row's last classes, one a thread.
+        for (int j = 0; j < p.k; ++j)
+          if (__builtin_amdgcn_readlane(entry.index, j) == shape.tail_class()) d.tail = -INFINITY;
+      }
+      if (seg == 0 && wave == 0) teacher_shares(p, row, entry, inv, sh);
+      float pm = d.tail;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) pm = fmaxf(pm, pack_max(d.pack[j]));
+      pm = wave_max(pm);
+      d.forget();
+      const float ref = fmaxf(pm, -FLT_MAX);
+      float part = __builtin_amdgcn_exp2f((d.tail - ref) * c);
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) part += __builtin_amdgcn_exp2f((d.pack[j].get(e) - ref) * c);
+      double ps = wave_sum((double)part);
+      if (ps != ps) pm = ref;  // a NaN is no maximum but must not be lost
+      if (pm > -INFINITY) {
+        const float nm = fmaxf(m, pm);
+        sum = (m == -INFINITY ? 0.0 : sum * (double)__builtin_amdgcn_exp2f((m - nm) * c)) +
+              ps * (double)__builtin_amdgcn_exp2f((pm - nm) * c);
+        m = nm;
+      }
+      if (PARTS) __syncthreads();  // the marks are no longer read
+    }
+    if (lane == 0) sh.max[wave] = m, sh.sum[wave] = sum;
+    __syncthreads();
+  }
+
+  float entry_grad = 0.0f;
+  if (wave == 0) {
+    if constexpr (MODE == kGradient) teacher_shares(p, row, entry, inv, sh);
+    const bool valid = entry.index >= 0;
+    const double q = sh.q[lane], q0 = sh.q0;
+    double top, z, mr, zr;
+    if constexpr (MODE == kGradient) {
+      const float* st = p.state + row * 4;
+      top = st[0], z = st[1], mr = st[2], zr = st[3];
+    } else {
+      const float om = lane < W ? sh.max[lane] : -INFINITY;
+      const float rm = wave_max(om);
+      zr = wave_sum(om > -INFINITY ? sh.sum[lane] * exp(((double)om - rm) * inv) : 0.0);
+      mr = rm;
+      top = fmaxf(rm, wave_max(valid ? own : -INFINITY));
+    }
+    const double low = fmax(top, -(double)FLT_MAX);
+    const double a = ((double)own - low) * inv;
+    const double e = valid ? exp(a) : 0.0;
+    const double e0 = mr == -INFINITY ? 0.0 : exp((mr - low) * inv);  // of the rest's maximum
+    if constexpr (MODE != kGradient) {
+      z = wave_sum(e) + zr * e0;
+      const double logz = log(z);
+      double term = valid && q > 0.0 ? q * (sh.logq[lane] - (a - logz)) : 0.0;
+      if (lane == 0 && q0 > 0.0)
+        term += q0 * (sh.logq0 - (zr > 0.0 || zr != zr ? (mr - low) * inv + log(zr) - logz : -INFINITY));
+      const double loss = wave_sum(term) * (double)p.temperature * (double)p.temperature;
+      if (lane == 0) {
+        p.loss[row] = top == -INFINITY && !(z != z) ? INFINITY : (float)loss;
+        if (MODE == kLoss && p.state) {
+          p.state[row * 4 + 0] = (float)top;
+          p.state[row * 4 + 1] = (float)z;
+          p.state[row * 4 + 2] = (float)mr;
+          p.state[row * 4 + 3] = (float)zr;
+        }
+      }
+    }
+    if constexpr (MODE != kLoss) {
+      const double scale = (p.grad_loss ? (double)p.grad_loss[row] : 1.0) * (double)p.temperature;
+      // No class has any probability: no gradient.
+      const bool dead = top == -INFINITY && !(z != z);
+      // Of exponentials relative to the rest's maximum: its classes may be far
+      // below the entries and still share q0 among them.
+      const double factor = dead || zr == 0.0 ? 0.0 : scale * (e0 / z - q0 / zr);
+      entry_grad = dead ? 0.0f : (float)(scale * (e / z - q));
+      if (lane == 0) sh.factor = (float)factor, sh.top = (float)fmax(mr, -(double)FLT_MAX);
+    }
+  }
+  if constexpr (MODE != kLoss) {
+    __syncthreads();
+    const float factor = sh.factor, ref = sh.top;
+    d.forget();
+    for (int seg = segs - 1; seg >= 0; --seg) {
+      if (PARTS) load_part(d, x, shape, seg);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = (seg * PER + j) * NT + tid;
+        if (i >= shape.full) continue;
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = factor * __builtin_amdgcn_exp2f((d.pack[j].get(e) - ref) * c);
+        Pack<T>::store(g + i * N, v);
+      }
+      if (seg == 0 && shape.has_tail())
+        st1<T>(g + shape.tail_class(), factor * __builtin_amdgcn_exp2f((d.tail - ref) * c));
+    }
+    __syncthreads();
+    if (wave == 0 && entry.index >= 0) st1<T>(g + entry.index, entry_grad);
+  }
+}
+
+template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
+void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  constexpr int kClasses = NT * PER * Pack<T>::N;
+  hipLaunchKernelGGL((distill_kernel<T, NT, PER, PARTS, MODE>), dim3((unsigned)in.rows), dim3(NT), 0, s, in, p,
+                     (in.classes + kClasses - 1) / kClasses);
+}
+
+// Threads of a row's workgroup and the elements that each holds.
+template <typename T, DistillMode MODE>
+void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  constexpr int N = Pack<T>::N;
+  if (in.rows < 512 && in.classes > 256 * 8 && in.classes <= 1024 * 32)
+    launch_distill_one<T, 1024, 32 / N, false, MODE>(in, p, s);
+  else if (in.classes <= 256 * 32)
+    launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
+  else if (in.classes <= 256 * 80)
+    launch_distill_one<T, 256, 80 / N, false, MODE>(in, p, s);
+  else
+    launch_distill_one<T, 1024, 80 / N, true, MODE>(in, p, s);
+}
+
+template <DistillMode MODE>
+void launch_distill_mode(const LogitRows& in, const DistillParams& p, hipStream_t s) {
+  in.dt == DT_BF16 ? launch_distill_typed<bf16, MODE>(in, p, s) : launch_distill_typed<float, MODE>(in, p, s);
+}
+
+}  // namespace
+
+void launch_distill(const LogitRows& student, const DistillParams& p, hipStream_t s) {
+  p.grad ? launch_distill_mode<kBoth>(student, p, s) : launch_distill_mode<kLoss>(student, p, s);
+}
+
+void launch_distill_grad(const LogitRows& student, const DistillParams& p, hipStream_t s) {
+  launch_distill_mode<kGradient>(student, p, s);
+}
+
+}  // namespace ppocr

@@ -1,0 +1,281 @@
+// Device code shared by the operators on rows of class logits: 16-byte packs,
+// rows held in registers, the rules of a row, wave reductions.
+#pragma once
+
+#include <cfloat>
+
+#include "device_math.h"
+#include "logits.h"
+
+namespace ppocr {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------- reductions
+// Data-parallel moves within a wave (row shifts by 1, 2, 4 and 8, then the
+// last lane of 16 and of 32 to the lanes behind): a few cycles a step, where
+// a shuffle goes through LDS.  The whole wave must be active.  Lanes without
+// a source keep `old`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_move(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <typename F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t none, F&& f) {
+#define STEP(CTRL, ROWS) v = f(v, (uint32_t)dpp_move<CTRL, ROWS>((int)none, (int)v))
+  STEP(0x111, 0xf);
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);
+  STEP(0x143, 0xc);
+#undef STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  return wave_reduce(v, 0, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+  return wave_reduce(v, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return __uint_as_float(wave_reduce(__float_as_uint(v), __float_as_uint(-INFINITY), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#define STEP(CTRL, ROWS)                                                                \
+  {                                                                                     \
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);                                 \
+    const uint32_t lo = (uint32_t)dpp_move<CTRL, ROWS>(0, (int)(uint32_t)u);            \
+    const uint32_t hi = (uint32_t)dpp_move<CTRL, ROWS>(0, (int)(uint32_t)(u >> 32));    \
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                           \
+  }
+  STEP(0x111, 0xf)
+  STEP(0x112, 0xf)
+  STEP(0x114, 0xf)
+  STEP(0x118, 0xf)
+  STEP(0x142, 0xa)
+  STEP(0x143, 0xc)
+#undef STEP
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// ------------------------------------------------------------------ packs
+// 16 bytes of a row, at any alignment of the element.
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+  static constexpr int N = 4;
+  typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const Raw r = *reinterpret_cast<const Raw*>(p);
+    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    *reinterpret_cast<Raw*>(p) = Raw{v[0], v[1], v[2], v[3]};
+  }
+};
+template <>
+struct Pack<bf16> {
+  static constexpr int N = 8;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
+  static __device__ __forceinline__ void load(const bf16* p, uint32_t (&v)[4]) {
+    const Raw r = *reinterpret_cast<const Raw*>(p);
+    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  }
+  static __device__ __forceinline__ void load(const bf16* p, float (&v)[8]) {
+    uint32_t r[4];
+    load(p, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float (&v)[8]) {
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<Raw*>(p) = r;
+  }
+};
+
+// One pack in registers: fp32, or bf16 as stored (half the registers; each
+// use widens it with one operation), which cannot hold what rules make of it.
+template <typename T, bool RAW>
+struct PackRegs {
+  static constexpr int N = Pack<T>::N;
+  float v[N];
+  __device__ __forceinline__ void load(const T* p) { Pack<T>::load(p, v); }
+  __device__ __forceinline__ float get(int e) const { return v[e]; }
+  __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
+  __device__ __forceinline__ void clear(int e) { v[e] = -INFINITY; }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = -INFINITY;
+  }
+  __device__ __forceinline__ void forget() {}
+};
+template <>
+struct PackRegs<bf16, true> {
+  static constexpr int N = 8;
+  uint32_t v[4];
+  __device__ __forceinline__ void load(const bf16* p) { Pack<bf16>::load(p, v); }
+  __device__ __forceinline__ float get(int e) const {
+    return __uint_as_float(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
+  }
+  __device__ __forceinline__ void clear(int e) {
+    v[e >> 1] = e & 1 ? (v[e >> 1] & 0xFFFFu) | 0xFF800000u : (v[e >> 1] & 0xFFFF0000u) | 0xFF80u;
+  }
+  __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0xFF80FF80u; }
+  // Widened values are not kept past here: twice the registers would be live.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("" : "+v"(v[i]));
+  }
+};
+template <typename P>
+__device__ __forceinline__ float pack_max(const P& p) {
+  float m = p.get(0);
+#pragma unroll
+  for (int e = 1; e < P::N; ++e) m = fmaxf(m, p.get(e));
+  return m;
+}
+
+// ------------------------------------------------------------------- rows
+// A part of a row in the registers of NT threads: PER packs each, in rounds of
+// NT packs, and one class of the row's last classes % N (with part 0; -inf
+// elsewhere).  Packs are numbered in the order that decides between equal
+// logits: from the row's start, or from its end when `last` is set.
+template <typename T, int NT, int PER, bool RAW>
+struct RowPart {
+  static constexpr int N = Pack<T>::N, kThreads = NT, kPer = PER, kClasses = NT * PER * N;
+  PackRegs<T, RAW> pack[PER];
+  float tail;
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) pack[j].forget();
+  }
+};
+template <int N>
+struct RowShape {
+  int classes, full, last;
+  __device__ __forceinline__ RowShape(int classes, int last) : classes(classes), full(classes / N), last(last) {}
+  __device__ __forceinline__ int pack_class(int i) const { return (last ? full - 1 - i : i) * N; }
+  __device__ __forceinline__ int tail_class() const { return full * N + (int)threadIdx.x; }
+  __device__ __forceinline__ bool has_tail() const { return tail_class() < classes; }
+  // Places in the order: packs, and the single classes behind or before them.
+  __device__ __forceinline__ int pack_place(int i) const { return i + N; }
+  __device__ __forceinline__ int tail_place() const {
+    return last ? classes - 1 - tail_class() : full + N + (int)threadIdx.x;
+  }
+};
+
+// Reads part `seg`; classes past the row are -inf.
+template <typename P, typename T, int N>
+__device__ __forceinline__ void load_part(P& d, const T* x, const RowShape<N>& s, int seg) {
+#pragma unroll
+  for (int j = 0; j < P::kPer; ++j) {
+    const int i = (seg * P::kPer + j) * P::kThreads + (int)threadIdx.x;
+    if (i < s.full)
+      d.pack[j].load(x + s.pack_class(i));
+    else
+      d.pack[j].clear();
+  }
+  d.tail = seg == 0 && s.has_tail() ? ld1<T>(x + s.tail_class()) : -INFINITY;
+}
+
+// ------------------------------------------------------------------ rules
+// A row of a rule table: the index given for the row, or table 0 of one, or the
+// row's own.  -1 outside the table: no rule.
+__device__ __forceinline__ int64_t table_row(const int32_t* index, int64_t n, int64_t row) {
+  const int64_t i = index ? (int64_t)index[row] : (n == 1 ? 0 : row);
+  return i >= 0 && i < n ? i : -1;
+}
+
+// One row's rules, in registers.
+struct RowRules {
+  const float* bias;
+  const uint32_t* mask;
+  const int32_t* history;
+  int n_history;
+  float repetition, frequency, presence;
+};
+
+__device__ __forceinline__ RowRules row_rules(const RuleParams& p, int64_t row, int classes) {
+  RowRules r;
+  r.bias = nullptr;
+  if (p.bias) {
+    const int64_t i = table_row(p.row_bias, p.n_bias, row);
+    if (i >= 0) r.bias = p.bias + i * classes;
+  }
+  r.mask = nullptr;
+  if (p.masks) {
+    const int64_t i = table_row(p.row_mask, p.n_masks, row);
+    if (i >= 0) r.mask = p.masks + i * ((classes + 31) / 32);
+  }
+  r.history = nullptr;
+  r.n_history = 0;
+  r.repetition = 1.0f, r.frequency = 0.0f, r.presence = 0.0f;
+  if (p.history) {
+    // Offsets come from device memory: kept inside the history.
+    const int64_t lo = min(max(p.offsets[row], (int64_t)0), p.history_len);
+    const int64_t hi = min(max(p.offsets[row + 1], lo), p.history_len);
+    r.history = p.history + lo;
+    r.n_history = (int)min(hi - lo, (int64_t)INT32_MAX);
+    if (p.repetition) r.repetition = p.repetition[row];
+    if (p.frequency) r.frequency = p.frequency[row];
+    if (p.presence) r.presence = p.presence[row];
+  }
+  return r;
+}
+
+// The penalties of a class that stands n > 0 times in the history, every step
+// rounded to fp32 by itself.
+__device__ __forceinline__ float penalise(const RowRules& r, float x, int n) {
+#pragma clang fp contract(off)
+  x = x > 0.0f ? x / r.repetition : x * r.repetition;
+  const float f = r.frequency * (float)n;
+  return x - (f + r.presence);
+}
+// Allowed classes c .. c + N - 1 (c a multiple of N) as N bits.
+template <int N>
+__device__ __forceinline__ unsigned mask_bits(const uint32_t* mask, int c) {
+  const unsigned b = reinterpret_cast<const uint8_t*>(mask)[c >> 3];
+  return N == 8 ? b : (b >> (c & 4)) & 15u;
+}
+__device__ __forceinline__ bool mask_bit(const uint32_t* mask, int c) { return mask[c >> 5] >> (c & 31) & 1; }
+// N biases from a table's row.
+template <int N>
+__device__ __forceinline__ void load_bias(const float* p, float (&v)[N]) {
+#pragma unroll
+  for (int q = 0; q < N; q += 4) {
+    float b[4];
+    Pack<float>::load(p + q, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[q + e] = b[e];
+  }
+}
+__device__ __forceinline__ float apply_rules(const RowRules& r, float x, int c, int n) {
+  if (n > 0) x = penalise(r, x, n);
+  if (r.bias) x = x + r.bias[c];
+  return r.mask && !mask_bit(r.mask, c) ? -INFINITY : x;
+}
+
+// Counts of the classes [first, first + n) in the row's history.
+__device__ __forceinline__ void count_history(const RowRules& r, int first, int n, int* counts) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < r.n_history; i += blockDim.x) {
+    const int c = r.history[i] - first;
+    if (c >= 0 && c < n) atomicAdd(&counts[c], 1);
+  }
+  __syncthreads();
+}
+
+}  // namespace ppocr

@@ -1,6 +1,7 @@
-// Parameter blocks and launchers of the operators on rows of class logits
-// (logits.hip): rules, top classes, distillation.  All pointers are device
-// memory; the C entry points (operators.cpp) have checked the shapes.
+// Parameter blocks and launchers of the operators on rows of class logits:
+// rules (logit_rules.hip), top classes (top_logits.hip), distillation
+// (distill.hip).  All pointers are device memory; the C entry points
+// (operators.cpp) have checked the shapes.
 #pragma once
 
 #include <hip/hip_runtime.h>

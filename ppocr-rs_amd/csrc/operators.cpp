@@ -1,4 +1,4 @@
-// C entry points of the operators on rows of class logits (logits.hip): the
+// C entry points of the operators on rows of class logits (logits.h): the
 // argument checks, the context's device and the launch.  Nothing here
 // allocates, waits or keeps state, so calls may run at once and be captured.
 #include <algorithm>
