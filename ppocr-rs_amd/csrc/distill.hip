@@ -49,7 +49,7 @@ struct DistillShared {
 template <typename T, int NT, int PER, bool PARTS>
 constexpr int distill_waves() {
   constexpr int regs = PER * 4;
-  return NT == 1024 && PARTS ? 4 : regs <= 16 ? 8 : regs <= 40 ? 6 : 4;
+  return NT == 1024 && PARTS ? 4 : regs <= 16 ? 8 : regs <= 40 ? 5 : 4;
 }
 
 // The teacher's shares of a row and their logs, by wave 0, in 64 bits: the loss
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
   const T* x = static_cast<const T*>(s.x) + row * s.stride;
   T* g = static_cast<T*>(p.grad) + row * p.grad_stride;
   TeacherEntry entry = teacher_entry(p, row, s.classes);
-  if (!__any(entry.index >= 0)) {
+  if (!lanes_where(entry.index >= 0)) {
     if (MODE != kGradient && tid == 0) p.loss[row] = 0.0f;
     if (MODE == kLoss && p.state && tid < 4) p.state[row * 4 + tid] = 0.0f;
     if (MODE != kLoss) {
@@ -130,31 +130,16 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
             for (int e = 0; e < N; ++e)
               if (word >> (q * 8 + e) & 1) d.pack[w * 4 + q].clear(e);
       }
-      if (seg == 0 && __any(entry.index >= shape.full * N)) {
+      if (seg == 0 && 0 != lanes_where(entry.index >= shape.full * N)) {
         // Entries among the row's last classes, one a thread.
         for (int j = 0; j < p.k; ++j)
           if (__builtin_amdgcn_readlane(entry.index, j) == shape.tail_class()) d.tail = -INFINITY;
       }
       if (seg == 0 && wave == 0) teacher_shares(p, row, entry, inv, sh);
-      float pm = d.tail;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) pm = fmaxf(pm, pack_max(d.pack[j]));
-      pm = wave_max(pm);
-      d.forget();
-      const float ref = fmaxf(pm, -FLT_MAX);
-      float part = __builtin_amdgcn_exp2f((d.tail - ref) * c);
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-#pragma unroll
-        for (int e = 0; e < N; ++e) part += __builtin_amdgcn_exp2f((d.pack[j].get(e) - ref) * c);
-      double ps = wave_sum((double)part);
-      if (ps != ps) pm = ref;  // a NaN is no maximum but must not be lost
-      if (pm > -INFINITY) {
-        const float nm = fmaxf(m, pm);
-        sum = (m == -INFINITY ? 0.0 : sum * (double)__builtin_amdgcn_exp2f((m - nm) * c)) +
-              ps * (double)__builtin_amdgcn_exp2f((pm - nm) * c);
-        m = nm;
-      }
+      float pm = part_max(d);
+      const double ps = part_sum(d, fmaxf(pm, -FLT_MAX), c);
+      if (ps != ps) pm = fmaxf(pm, -FLT_MAX);  // a NaN is no maximum but must not be lost
+      join_sums(m, sum, pm, ps, c);
       if (PARTS) __syncthreads();  // the marks are no longer read
     }
     if (lane == 0) sh.max[wave] = m, sh.sum[wave] = sum;
@@ -215,6 +200,8 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
     d.forget();
     for (int seg = segs - 1; seg >= 0; --seg) {
       if (PARTS) load_part(d, x, shape, seg);
+      // By the difference: this loop's two forms would share their addresses,
+      // which then take the registers.
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         const int i = (seg * PER + j) * NT + tid;
@@ -243,8 +230,8 @@ void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t
 template <typename T, DistillMode MODE>
 void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N;
-  if (in.rows < 512 && in.classes > 256 * 8 && in.classes <= 1024 * 32)
-    launch_distill_one<T, 1024, 32 / N, false, MODE>(in, p, s);
+  if (in.rows < 1024 && in.classes > 256 * 8 && in.classes <= 512 * 40)
+    launch_distill_one<T, 512, 40 / N, false, MODE>(in, p, s);
   else if (in.classes <= 256 * 32)
     launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
   else if (in.classes <= 256 * 80)

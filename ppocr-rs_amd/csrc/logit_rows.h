@@ -12,6 +12,10 @@ namespace ppocr {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------- reductions
+// Lanes where v holds (the compare's own result; HIP's __ballot makes an
+// integer of it first).
+__device__ __forceinline__ uint64_t lanes_where(bool v) { return __builtin_amdgcn_ballot_w64(v); }
+
 // Data-parallel moves within a wave (row shifts by 1, 2, 4 and 8, then the
 // last lane of 16 and of 32 to the lanes behind): a few cycles a step, where
 // a shuffle goes through LDS.  The whole wave must be active.  Lanes without
@@ -119,6 +123,7 @@ struct PackRegs {
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = -INFINITY;
   }
+  template <int AT = 0>
   __device__ __forceinline__ void forget() {}
 };
 template <>
@@ -134,9 +139,11 @@ struct PackRegs<bf16, true> {
   }
   __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0xFF80FF80u; }
   // Widened values are not kept past here: twice the registers would be live.
+  // (AT tells two branches apart, whose beginnings would be joined.)
+  template <int AT = 0>
   __device__ __forceinline__ void forget() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) asm("" : "+v"(v[i]));
+    for (int i = 0; i < 4; ++i) asm volatile("; %1" : "+v"(v[i]) : "n"(AT));
   }
 };
 template <typename P>
@@ -157,9 +164,10 @@ struct RowPart {
   static constexpr int N = Pack<T>::N, kThreads = NT, kPer = PER, kClasses = NT * PER * N;
   PackRegs<T, RAW> pack[PER];
   float tail;
+  template <int AT = 0>
   __device__ __forceinline__ void forget() {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) pack[j].forget();
+    for (int j = 0; j < PER; ++j) pack[j].template forget<AT>();
   }
 };
 template <int N>
@@ -188,6 +196,60 @@ __device__ __forceinline__ void load_part(P& d, const T* x, const RowShape<N>& s
       d.pack[j].clear();
   }
   d.tail = seg == 0 && s.has_tail() ? ld1<T>(x + s.tail_class()) : -INFINITY;
+}
+
+// exp((x - m) / tau) for many x: 2^(x c - b) with c = log2(e) / tau and b = m c
+// rounded, one fused operation and the hardware exponential.  What b's rounding
+// leaves out, the same factor of every term, is `fix` (within 3% of one): sums
+// and products take it once.  A reference so large that b would have no fraction
+// left (rows at a type's lowest value, infinities) goes by the difference.
+struct ExpFrom {
+  float m, c, b, fix;
+  bool far;
+  __device__ __forceinline__ ExpFrom(float m, float c) : m(m), c(c), b(m * c) {
+    far = !(fabsf(b) < 1048576.0f);
+    fix = far ? 1.0f : __builtin_amdgcn_exp2f(-fmaf(m, c, -b));
+  }
+  template <bool FAR>
+  __device__ __forceinline__ float term(float x) const {
+    return __builtin_amdgcn_exp2f(FAR ? (x - m) * c : fmaf(x, c, -b));
+  }
+};
+
+// Sum of the terms of a part (without `fix`).
+template <bool FAR, typename P>
+__device__ __forceinline__ float part_terms(P& d, const ExpFrom& from) {
+  d.template forget<FAR>();
+  float s = from.term<FAR>(d.tail);
+#pragma unroll
+  for (int j = 0; j < P::kPer; ++j)
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) s += from.term<FAR>(d.pack[j].get(e));
+  return s;
+}
+// The wave's sum of exp((x - m) / tau) over a part.
+template <typename P>
+__device__ __forceinline__ double part_sum(P& d, float m, float c) {
+  const ExpFrom from(m, c);
+  const float s = from.far ? part_terms<true>(d, from) : part_terms<false>(d, from);
+  return wave_sum((double)s) * (double)from.fix;
+}
+template <typename P>
+__device__ __forceinline__ float part_max(const P& d) {
+  float m = d.tail;
+#pragma unroll
+  for (int j = 0; j < P::kPer; ++j) m = fmaxf(m, pack_max(d.pack[j]));
+  return wave_max(m);
+}
+
+// Sums of exp((x - max) * c) with their own maxima, joined: (m, s) becomes the
+// sum of both.  -inf is no maximum.
+__device__ __forceinline__ void join_sums(float& m, double& s, float om, double os, float c) {
+  const float nm = fmaxf(m, om);
+  if (nm == -INFINITY) return;
+  s = (m == -INFINITY ? 0.0 : s * (double)__builtin_amdgcn_exp2f((m - nm) * c)) +
+      (om == -INFINITY ? 0.0 : os * (double)__builtin_amdgcn_exp2f((om - nm) * c));
+  m = nm;
 }
 
 // ------------------------------------------------------------------ rules

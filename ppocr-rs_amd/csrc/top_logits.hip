@@ -102,63 +102,36 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
   if constexpr (RULES) rule_part(d, r, s, seg, counts);
 }
 
-// Sums of exp((x - max) * c) with their own maxima, joined: (m, s) becomes the
-// sum of both.  -inf is no maximum.
-__device__ __forceinline__ void join_sums(float& m, double& s, float om, double os, float c) {
-  const float nm = fmaxf(m, om);
-  if (nm == -INFINITY) return;
-  s = (m == -INFINITY ? 0.0 : s * (double)__builtin_amdgcn_exp2f((m - nm) * c)) +
-      (om == -INFINITY ? 0.0 : os * (double)__builtin_amdgcn_exp2f((om - nm) * c));
-  m = nm;
-}
-
-// The sum of exp((v - m) * c) over a part, m the wave's maximum of it, limited to
-// finite numbers: +inf then counts as an infinite term and -inf as none.
-template <typename P>
-__device__ __forceinline__ void part_sum(P& d, float c, float& m, double& sum) {
-  float t = d.tail;
-#pragma unroll
-  for (int j = 0; j < P::kPer; ++j) t = fmaxf(t, pack_max(d.pack[j]));
-  m = wave_max(t);
-  d.forget();
-  const float ref = fminf(fmaxf(m, -FLT_MAX), FLT_MAX);
-  float s = __builtin_amdgcn_exp2f((d.tail - ref) * c);
-#pragma unroll
-  for (int j = 0; j < P::kPer; ++j)
-#pragma unroll
-    for (int e = 0; e < P::N; ++e) s += __builtin_amdgcn_exp2f((d.pack[j].get(e) - ref) * c);
-  sum = wave_sum((double)s);
-  // A NaN is no maximum but must not be lost.
-  if (m == -INFINITY && sum != sum) m = -FLT_MAX;
-  m = fminf(m, FLT_MAX);
-}
-
 // The k best classes of a row and the log-sum-exp of the others, one row a
 // workgroup, the row read once (parts of longer rows a second time).
 //
 // Every group of NT / 256 threads has its best (logit, first place that holds
 // it).  The k-th best of the 256 groups bounds the k-th best class from below,
-// and only about k groups hold classes above the bound: those go to a list in
-// LDS, out of the registers, and each finds its rank by counting the better
-// ones.  What is left in the registers and the list's end is the rest.  The
-// bound is found by bisection over the groups' order keys, every wave for
-// itself.  A list that overflows (rows whose best classes crowd in few threads)
-// sends the row to k searches for the next best class.
-constexpr int kGroups = 256, kList = 512;
+// and only about k groups hold classes above the bound: those leave the
+// registers for a list of the wave in LDS, and each finds its rank by counting
+// the better ones in all lists.  What is left in the registers and the end of
+// the ranking is the rest.  The bound is found by bisection over the groups'
+// order keys, every wave for itself.  Lists that overflow (rows whose best
+// classes crowd in few threads) or a NaN (which shows in the sums) send the row
+// to k searches for the next best class.
+constexpr int kGroups = 256, kList = 256, kSorted = 512;
 
+template <int W>
 struct TopShared {
-  alignas(16) uint64_t list[kList];
-  uint64_t sorted[kList];
+  alignas(16) uint64_t list[W][kList];
+  uint64_t sorted[kSorted];
   uint32_t group_key[kGroups], group_place[kGroups];
   uint64_t red[16];
   double wave_sum[16];
   float wave_max[16];
-  int n_list;
+  int count[W];  // of the waves' lists
+  int nan;
 };
 
 // Bound of the list: the composite (value key, ~place) that at least k groups
 // reach, and few more.
-__device__ __forceinline__ uint64_t top_bound(const TopShared& sh, int k) {
+template <int W>
+__device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
   const int lane = threadIdx.x & 63;
   uint32_t key[4], place[4];
 #pragma unroll
@@ -166,7 +139,7 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared& sh, int k) {
   const auto reach = [&](uint32_t t) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= t));
+    for (int i = 0; i < 4; ++i) n += __popcll(lanes_where(key[i] >= t));
     return n;
   };
   if (reach(kNone + 1) <= k) return (uint64_t)(kNone + 1) << 32;
@@ -193,7 +166,7 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared& sh, int k) {
     const uint32_t mid = plo + (phi - plo) / 2;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c += __popcll(__ballot(key[i] == lo && place[i] >= mid));
+    for (int i = 0; i < 4; ++i) c += __popcll(lanes_where(key[i] == lo && place[i] >= mid));
     if (c >= need)
       plo = mid;
     else
@@ -204,9 +177,9 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared& sh, int k) {
 
 // The slow way for any row: k searches for the best class below the last one,
 // then the sums of the others, the row read each time.
-template <typename T, bool RULES>
+template <typename T, bool RULES, int W>
 __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int classes, const TopParams& p, float c,
-                                           int* counts, TopShared& sh, float& wm, double& ws) {
+                                           int* counts, TopShared<W>& sh, float& wm, double& ws) {
   const auto each = [&](auto&& f) {
     for (int first = 0; first < classes; first += kWindow) {
       const int n = min(kWindow, classes - first);
@@ -242,7 +215,7 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
   each([&](float v, uint64_t key) {
     if (key < last) sum += (double)__builtin_amdgcn_exp2f((v - m) * c);
   });
-  wm = __any(some) ? m : -INFINITY;
+  wm = 0 != lanes_where(some) ? m : -INFINITY;
   ws = wave_sum(sum);
 }
 
@@ -250,13 +223,13 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
 template <typename T, int NT, int PER, bool RULES>
 constexpr int top_waves() {
   constexpr int regs = RULES ? PER * Pack<T>::N : PER * 4;
-  return NT == 1024 ? 4 : regs <= 32 ? RULES ? 5 : 7 : regs <= 40 ? 6 : RULES ? 3 : 4;
+  return NT == 1024 ? 4 : regs <= 32 ? RULES ? 5 : 7 : regs <= 40 ? 5 : RULES ? 3 : 4;
 }
 
 template <typename T, int NT, int PER, bool RULES>
 __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logits_kernel(LogitRows in, TopParams p, int parts) {
   constexpr int N = Pack<T>::N, W = NT / 64;
-  __shared__ TopShared sh;
+  __shared__ TopShared<W> sh;
   extern __shared__ int counts[];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
@@ -265,51 +238,33 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   if constexpr (RULES) r = row_rules(p.rules, row, in.classes);
   const RowShape<N> shape(in.classes, p.last_ties);
   const float c = kLog2e / p.temperature;
-  for (int i = tid; i < kList; i += NT) sh.list[i] = 0;
-  if (tid == 0) sh.n_list = 0;
+  if (tid == 0) sh.nan = 0;
 
   // Best logit of this thread and the first place that holds it.
   RowPart<T, NT, PER, !RULES> d;
+  float high[PER];  // each pack's maximum
   float best = -INFINITY;
   int place = 0;
-  bool nan = false;
-  int nan_place = 0;
   float tail = -INFINITY;
   const auto look = [&](float m, int at) {
     const bool better = m > best;
     best = better ? m : best;
     place = better ? at : place;
   };
-  const auto look_tail = [&] {
-    look(tail, shape.tail_place());
-    if (tail != tail && !nan) nan = true, nan_place = shape.tail_place();
-  };
   for (int seg = 0; seg < parts; ++seg) {
     read_part<RULES>(d, x, r, shape, seg, counts);
     if (seg == 0) {
       tail = d.tail;
-      if (shape.last) look_tail();
+      if (shape.last) look(tail, shape.tail_place());
     }
-    bool bad = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      look(pack_max(d.pack[j]), shape.pack_place((seg * PER + j) * NT + tid));
-#pragma unroll
-      for (int e = 0; e < N; e += 2) bad |= __builtin_isunordered(d.pack[j].get(e), d.pack[j].get(e + 1));
-    }
-    if (bad && !nan) {
-      nan = true;
-      nan_place = INT32_MAX;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (d.pack[j].get(e) != d.pack[j].get(e))
-            nan_place = min(nan_place, shape.pack_place((seg * PER + j) * NT + tid));
+      high[j] = pack_max(d.pack[j]);
+      look(high[j], shape.pack_place((seg * PER + j) * NT + tid));
     }
   }
-  if (!shape.last) look_tail();
-  uint64_t mine = (uint64_t)value_key(nan ? NAN : best) << 32 | (uint32_t)~(nan ? nan_place : place);
+  if (!shape.last) look(tail, shape.tail_place());
+  uint64_t mine = (uint64_t)value_key(best) << 32 | (uint32_t)~place;
   if constexpr (NT > kGroups) {
 #pragma unroll
     for (int o = 1; o < NT / kGroups; o <<= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
@@ -320,83 +275,74 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   }
   __syncthreads();
 
-  // Classes above the bound go to the list, one atomic a wave: count, reserve,
-  // write.  The others' sums.
+  // Classes above the bound go to the wave's list; the others' sums.
   const uint64_t bound = top_bound(sh, p.k);
   const float floor_value = key_value(bound);
-  d.forget();
+  const uint32_t floor_place = (uint32_t)bound;
   float wm = -INFINITY;
   double ws = 0.0;
+  int n_wave = 0;
+  d.forget();
   for (int seg = parts - 1; seg >= 0; --seg) {
-    if (seg != parts - 1) read_part<RULES>(d, x, r, shape, seg, counts);
-    const auto pass = [&](float v, int at) {
-      const uint32_t key = value_key(v);
-      return ((uint64_t)key << 32 | (uint32_t)~at) >= bound && key > kNone;
+    if (seg != parts - 1) {
+      read_part<RULES>(d, x, r, shape, seg, counts);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) high[j] = pack_max(d.pack[j]);
+    }
+    // A class passes above the bound's value, or at it in a place that the
+    // bound reaches; at least -FLT_MAX in any case.
+    const auto take = [&](float v, int at, int cls) {
+      uint64_t lanes = lanes_where(v >= floor_value);
+      if (!lanes) return false;
+      lanes &= lanes_where(v > floor_value) | lanes_where((uint32_t)~at >= floor_place);
+      const bool mine = lanes >> lane & 1;
+      const int slot = n_wave + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+      if (mine && slot < kList) sh.list[wave][slot] = order_key(v, cls, p.last_ties);
+      n_wave += __popcll(lanes);
+      return mine;
     };
-    int n = 0;
-    uint32_t hit = 0;  // packs with a class above the bound in some lane
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (__any(pack_max(d.pack[j]) >= floor_value || nan)) {
-        const int at = shape.pack_place((seg * PER + j) * NT + tid);
+      if (!lanes_where(high[j] >= floor_value)) continue;
+      const int i = (seg * PER + j) * NT + tid;
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (__any(!(d.pack[j].get(e) < floor_value))) {
-            n += __popcll(__ballot(pass(d.pack[j].get(e), at)));
-            hit |= 1u << j;
-          }
-      }
+      for (int e = 0; e < N; ++e)
+        if (take(d.pack[j].get(e), shape.pack_place(i), shape.pack_class(i) + e)) d.pack[j].clear(e);
+      high[j] = pack_max(d.pack[j]);
     }
-    const uint64_t tails = seg == 0 ? __ballot(pass(d.tail, shape.tail_place())) : 0;
-    n += __popcll(tails);
-    d.forget();
-    if (n) {
-      int slot = 0;
-      if (lane == 0) slot = atomicAdd(&sh.n_list, n);
-      slot = __builtin_amdgcn_readfirstlane(slot);
-      const auto put = [&](uint64_t lanes, float v, int cls) {
-        const int at = slot + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
-        const bool mine = lanes >> lane & 1;
-        if (mine && at < kList) sh.list[at] = order_key(v, cls, p.last_ties);
-        slot += __popcll(lanes);
-        return mine;
-      };
+    if (seg == 0 && take(d.tail, shape.tail_place(), shape.tail_class())) d.tail = -INFINITY;
+    float m = d.tail;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        if (hit >> j & 1) {
-          const int i = (seg * PER + j) * NT + tid;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float v = d.pack[j].get(e);
-            if (__any(!(v < floor_value)))
-              if (put(__ballot(pass(v, shape.pack_place(i))), v, shape.pack_class(i) + e)) d.pack[j].clear(e);
-          }
-        }
-      }
-      if (tails && put(tails, d.tail, shape.tail_class())) d.tail = -INFINITY;
-    }
-    d.forget();
-    float m;
-    double s;
-    part_sum(d, c, m, s);
-    join_sums(wm, ws, m, s, c);
+    for (int j = 0; j < PER; ++j) m = fmaxf(m, high[j]);
+    m = wave_max(m);
+    // The maximum limited to finite numbers: +inf then counts as an infinite
+    // term and -inf as none.
+    const double sum = part_sum(d, fminf(fmaxf(m, -FLT_MAX), FLT_MAX), c);
+    if (sum != sum) sh.nan = 1;
+    join_sums(wm, ws, fminf(m, FLT_MAX), sum, c);
   }
-  if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws;
+  if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws, sh.count[wave] = n_wave;
+  // Zeros behind the list, to the next eight.
+  if (lane < 8 && n_wave + lane < kList) sh.list[wave][n_wave + lane] = 0;
   __syncthreads();
 
-  int n = sh.n_list;
-  if (n <= kList) {
-    for (int i = tid; i < n; i += NT) {
-      const uint64_t key = sh.list[i];
-      int rank = 0;
-      // Eight keys at a time (zeros behind the last).
-      for (int o = 0; o < n; o += 8)
+  int n = 0, most = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) rank += sh.list[o + q] > key;
+  for (int w = 0; w < W; ++w) n += sh.count[w], most = max(most, sh.count[w]);
+  if (n <= kSorted && most <= kList && !sh.nan) {
+    for (int i = tid; i < n; i += NT) {
+      int from = 0, at = i;
+      while (at >= sh.count[from]) at -= sh.count[from++];
+      const uint64_t key = sh.list[from][at];
+      int rank = 0;
+      for (int w = 0; w < W; ++w)
+        for (int o = 0; o < sh.count[w]; o += 8)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) rank += sh.list[w][o + q] > key;
       sh.sorted[rank] = key;
     }
   } else {
-    search_row<T, RULES>(x, r, in.classes, p, c, counts, sh, wm, ws);
+    search_row<T, RULES, W>(x, r, in.classes, p, c, counts, sh, wm, ws);
     n = p.k;
     if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws;
   }
@@ -447,9 +393,8 @@ void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
 template <typename T, bool RULES>
 void launch_top_typed(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N, kLong = RULES ? 64 : 80;
-  if (in.rows < 512 && in.classes > 256 * 8)
-    in.classes <= 1024 * 32 ? launch_top<T, 1024, 32 / N, RULES>(in, p, s)
-                            : launch_top<T, 1024, kLong / N, RULES>(in, p, s);
+  if (in.rows < 1024 && in.classes > 256 * 8 && in.classes <= 512 * 40)
+    launch_top<T, 512, 40 / N, RULES>(in, p, s);
   else if (in.classes <= 256 * 32)
     launch_top<T, 256, 32 / N, RULES>(in, p, s);
   else if (in.classes <= 256 * 80)
