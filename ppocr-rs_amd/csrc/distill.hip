@@ -226,16 +226,22 @@ void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t
                      (in.classes + kClasses - 1) / kClasses);
 }
 
-// Threads of a row's workgroup and the elements that each holds.
+// Threads of a row's workgroup and the elements that each holds.  512 threads
+// of 40 elements keep more waves on a CU than 256 of 80 (2560 x 18710 fp32, loss
+// and gradient: 80 us against 105); the loss alone needs so few registers that
+// batches are even in fp32 and faster with 256 in bf16 (10240 x 18710: 98 us
+// against 109), but a few hundred rows fill the chip better with 512 (378 x
+// 18710 fp32: 9.3 us against 12.4).
 template <typename T, DistillMode MODE>
 void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N;
-  if (in.rows < 1024 && in.classes > 256 * 8 && in.classes <= 512 * 40)
+  const bool wide = in.rows < 1024 || (MODE != kLoss && in.classes > 256 * 32);
+  if (wide && in.classes > 256 * 8 && in.classes <= 512 * 40)
     launch_distill_one<T, 512, 40 / N, false, MODE>(in, p, s);
   else if (in.classes <= 256 * 32)
     launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
-  else if (in.classes <= 256 * 80)
-    launch_distill_one<T, 256, 80 / N, false, MODE>(in, p, s);
+  else if (MODE == kLoss && in.classes <= 256 * 80)
+    launch_distill_one<T, 256, 80 / N, false, kLoss>(in, p, s);
   else
     launch_distill_one<T, 1024, 80 / N, true, MODE>(in, p, s);
 }

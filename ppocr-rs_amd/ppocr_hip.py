@@ -277,6 +277,14 @@ def _torch():
     return _torch_module
 
 
+def _current_stream(device):
+    """The HIP stream that torch uses on the device."""
+    return _torch_module.cuda.current_stream(device).cuda_stream
+
+
+_ROW_TYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+
+
 def _rows(t, what):
     """``ppocr_logits`` of a tensor [..., classes] whose rows lie one stride apart."""
     if t.dim() < 1:
@@ -286,17 +294,23 @@ def _rows(t, what):
     rows, classes = t.shape
     if classes > 1 and t.stride(1) != 1:
         raise ValueError(f"{what}: the classes of a row must be adjacent")
-    kind = str(t.dtype)
-    if kind not in ("torch.float32", "torch.bfloat16"):
-        raise ValueError(f"{what} must be float32 or bfloat16, not {kind}")
-    return _Logits(t.data_ptr(), rows, classes, t.stride(0) if rows > 1 else max(classes, t.stride(0)),
-                   1 if kind == "torch.bfloat16" else 0)
+    kind = _ROW_TYPES.get(str(t.dtype))
+    if kind is None:
+        raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}")
+    return _Logits(t.data_ptr(), rows, classes, t.stride(0) if rows > 1 else max(classes, t.stride(0)), kind)
 
 
 def _rows_like(t, like, what):
     if t.shape != like.shape or t.dtype != like.dtype:
         raise ValueError(f"{what} must have the logits' shape and type")
     return _rows(t, what)
+
+
+def _output(torch, out, like, rows):
+    """The rows that a call writes and their stride: given, or new ones."""
+    if out is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format), rows.classes
+    return out, _rows_like(out, like, "out").stride
 
 
 def _packed(t, dtype, count, what):
@@ -457,18 +471,15 @@ class Gpu:
     # Operators on rows of class logits: torch tensors on this device, the
     # work queued on torch's current stream of the device.
 
-    def _stream(self):
-        return _torch().cuda.current_stream(self.device).cuda_stream
-
     def logit_rules(self, logits, rules, out=None):
         """Penalties, biases and masks of ``rules`` (LogitRules) on logits
         [..., classes] (float32 or bfloat16); ``out`` may be the logits."""
+        torch = _torch()
         rows = _rows(logits, "logits")
         rules.check(rows.rows)
-        if out is None:
-            out = _torch().empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        o = _rows_like(out, logits, "out")
-        _check(lib().ppocr_hip_logit_rules(self.handle, rows, rules.struct, o.data, o.stride, self._stream()))
+        out, stride = _output(torch, out, logits, rows)
+        _check(_lib.ppocr_hip_logit_rules(self.handle, rows, rules.struct, out.data_ptr(), stride,
+                                          _current_stream(self.device)))
         return out
 
     def top_logits(self, logits, k, rules=None, temperature=1.0):
@@ -482,9 +493,9 @@ class Gpu:
         values = torch.empty((*lead, int(k)), dtype=torch.float32, device=logits.device)
         indices = torch.empty((*lead, int(k)), dtype=torch.int32, device=logits.device)
         rest = torch.empty(lead, dtype=torch.float32, device=logits.device)
-        _check(lib().ppocr_hip_top_logits(self.handle, rows, rules.struct if rules is not None else None, int(k),
-                                          temperature, values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
-                                          self._stream()))
+        _check(_lib.ppocr_hip_top_logits(self.handle, rows, rules.struct if rules is not None else None, int(k),
+                                         temperature, values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
+                                         _current_stream(self.device)))
         return TopLogits(values, indices, rest)
 
     def distill_loss(self, student, teacher, temperature=1.0):
@@ -496,21 +507,20 @@ class Gpu:
         lead = student.shape[:-1]
         loss = torch.empty(lead, dtype=torch.float32, device=student.device)
         state = torch.empty((*lead, 4), dtype=torch.float32, device=student.device)
-        _check(lib().ppocr_hip_distill_loss(self.handle, rows, t, temperature, loss.data_ptr(), state.data_ptr(),
-                                            self._stream()))
+        _check(_lib.ppocr_hip_distill_loss(self.handle, rows, t, temperature, loss.data_ptr(), state.data_ptr(),
+                                           _current_stream(self.device)))
         return loss, state
 
     def distill_grad(self, student, teacher, state, temperature=1.0, grad_loss=None, out=None):
         """Gradient of ``sum(grad_loss * loss)`` by the student's logits, from
         the state that ``distill_loss`` left; ``out`` may be the logits."""
+        torch = _torch()
         rows = _rows(student, "student")
         t = _teacher(teacher, rows.rows)
-        if out is None:
-            out = _torch().empty(student.shape, dtype=student.dtype, device=student.device)
-        o = _rows_like(out, student, "out")
-        _check(lib().ppocr_hip_distill_grad(self.handle, rows, t, _packed(state, "float32", rows.rows * 4, "state"),
-                                            temperature, _packed(grad_loss, "float32", rows.rows, "grad_loss"),
-                                            o.data, o.stride, self._stream()))
+        out, stride = _output(torch, out, student, rows)
+        _check(_lib.ppocr_hip_distill_grad(self.handle, rows, t, _packed(state, "float32", rows.rows * 4, "state"),
+                                           temperature, _packed(grad_loss, "float32", rows.rows, "grad_loss"),
+                                           out.data_ptr(), stride, _current_stream(self.device)))
         return out
 
     def distill(self, student, teacher, temperature=1.0, grad_loss=None, out=None):
@@ -520,12 +530,10 @@ class Gpu:
         rows = _rows(student, "student")
         t = _teacher(teacher, rows.rows)
         loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=student.device)
-        if out is None:
-            out = torch.empty(student.shape, dtype=student.dtype, device=student.device)
-        o = _rows_like(out, student, "out")
-        _check(lib().ppocr_hip_distill(self.handle, rows, t, temperature,
-                                       _packed(grad_loss, "float32", rows.rows, "grad_loss"), loss.data_ptr(),
-                                       o.data, o.stride, self._stream()))
+        out, stride = _output(torch, out, student, rows)
+        _check(_lib.ppocr_hip_distill(self.handle, rows, t, temperature,
+                                      _packed(grad_loss, "float32", rows.rows, "grad_loss"), loss.data_ptr(),
+                                      out.data_ptr(), stride, _current_stream(self.device)))
         return loss, out
 
     def close(self):
