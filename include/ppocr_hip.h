@@ -107,10 +107,47 @@ ppocr_status ppocr_hip_recognizer_load_greedy(ppocr_hip_ctx* ctx, const char* sa
                                               ppocr_model_size size, const size_t nchw[4], ppocr_precision precision,
                                               const ppocr_hip_model* share_weights, ppocr_hip_model** out);
 
+/* Rules on a recognizer's classes, in host memory (copied by the calls that
+ * take them): `bias` [classes] is added to the logits (finite values), and bit
+ * c % 32 of word c / 32 of `allowed` [ceil(classes / 32)] tells whether class c
+ * may be answered (the blank, class 0, always may: it must be set).  Either may
+ * be NULL. */
+typedef struct ppocr_class_rules {
+  size_t classes; /* of the recognizer: 6906 (tiny) or 18710 */
+  const float* bias;
+  const uint32_t* allowed;
+} ppocr_class_rules;
+
+typedef enum ppocr_recognizer_output {
+  PPOCR_OUTPUT_PROBABILITIES = 0, /* [N, T, V], as ppocr_hip_recognizer_load */
+  PPOCR_OUTPUT_GREEDY = 1,        /* [N, T, 2], as ppocr_hip_recognizer_load_greedy */
+  PPOCR_OUTPUT_TOP = 2            /* [N, T, top_k, 2]: the best classes of each time step */
+} ppocr_recognizer_output;
+
+typedef struct ppocr_recognizer_options {
+  ppocr_recognizer_output output;
+  size_t top_k;                   /* 1 to 64 with PPOCR_OUTPUT_TOP, else 0 */
+  const ppocr_class_rules* rules; /* NULL: none */
+} ppocr_recognizer_options;
+
+/* A recognizer with one of three outputs, and with rules on its classes
+ * (lines of digits, one script, a lexicon's classes preferred).  The softmax is
+ * over the allowed classes' biased logits; a class that is not allowed has
+ * probability 0.  PPOCR_OUTPUT_TOP gives each time step's top_k classes and
+ * probabilities, largest first (equal ones: the highest class first, as greedy
+ * decoding takes them), as candidates for a search over a lexicon; where fewer
+ * classes are allowed the places left hold (-1, 0).  Without rules and with the
+ * first two outputs this is ppocr_hip_recognizer_load and
+ * ppocr_hip_recognizer_load_greedy.  No counterpart in the reference. */
+ppocr_status ppocr_hip_recognizer_load_with(ppocr_hip_ctx* ctx, const char* safetensors_path, ppocr_model_size size,
+                                            const size_t nchw[4], ppocr_precision precision,
+                                            const ppocr_recognizer_options* options,
+                                            const ppocr_hip_model* share_weights, ppocr_hip_model** out);
+
 void ppocr_hip_model_free(ppocr_hip_model* model);
 
 /* Output shape of `ModelOutput` (src/gpu/model.rs:37-41): detector
- * [N, 1, H, W] (rank 4), recognizer [N, T, V] (rank 3). */
+ * [N, 1, H, W] (rank 4), recognizer [N, T, V] (rank 3) or its other outputs'. */
 ppocr_status ppocr_hip_output_shape(const ppocr_hip_model* model, size_t shape[4], size_t* rank);
 
 /* Replaces `Detector::forward` / `Recognizer::forward`
@@ -301,6 +338,11 @@ ppocr_status ppocr_hip_engine_load(ppocr_hip_ctx* ctx, const char* detector_path
                                    size_t dictionary_len, const ppocr_engine_options* options,
                                    ppocr_hip_engine** out);
 void ppocr_hip_engine_free(ppocr_hip_engine* engine);
+
+/* Rules on the classes of every line that the engine recognises from here on
+ * (NULL: none, as loaded).  Recognizer plans loaded so far are dropped.  No
+ * counterpart in the reference. */
+ppocr_status ppocr_hip_engine_set_rules(ppocr_hip_engine* engine, const ppocr_class_rules* rules);
 
 /* `OcrEngine::recognize` / `recognize_with` (src/ocr.rs:497-600) on an RGB8
  * image (row-major HWC, width * height * 3 bytes).  The result is read with

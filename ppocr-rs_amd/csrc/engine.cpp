@@ -114,6 +114,8 @@ struct ppocr_hip_engine {
   std::vector<Cached> detectors, recognizers;
   ppocr_hip_model* shared_weights = nullptr;  // any live recognizer plan
   PinnedStage stage;
+  std::vector<float> rule_bias;  // class rules of the recognizers (empty: none)
+  std::vector<uint32_t> rule_allowed;
   ~ppocr_hip_engine() {
     // Queued downloads may still target the staging area and queued graphs
     // may still run the cached plans.
@@ -147,6 +149,12 @@ ppocr_hip_model* cached_model(ppocr_hip_engine* e, std::vector<Cached>& cache, s
   const ppocr_engine_options& o = e->options;
   if (detector) {
     check(ppocr_hip_detector_load(e->ctx, e->detector_path.c_str(), o.detector_size, shape, o.precision, &m));
+  } else if (!e->rule_bias.empty() || !e->rule_allowed.empty()) {
+    const ppocr_class_rules rules{e->classes, e->rule_bias.empty() ? nullptr : e->rule_bias.data(),
+                                  e->rule_allowed.empty() ? nullptr : e->rule_allowed.data()};
+    const ppocr_recognizer_options with{o.greedy ? PPOCR_OUTPUT_GREEDY : PPOCR_OUTPUT_PROBABILITIES, 0, &rules};
+    check(ppocr_hip_recognizer_load_with(e->ctx, e->recognizer_path.c_str(), o.recognizer_size, shape, o.precision,
+                                         &with, e->shared_weights, &m));
   } else if (o.greedy) {
     check(ppocr_hip_recognizer_load_greedy(e->ctx, e->recognizer_path.c_str(), o.recognizer_size, shape,
                                            o.precision, e->shared_weights, &m));
@@ -208,7 +216,7 @@ ppocr_status ppocr_hip_engine_load(ppocr_hip_ctx* ctx, const char* detector_path
     ppocr::db_options(&o.postprocess);
     if (o.precision != PPOCR_F32 && o.precision != PPOCR_BF16) ppocr::raise(PPOCR_ERR_INVALID_INPUT, "unknown precision");
     // validate_recognizer_dictionary (src/ocr.rs:691-700).
-    e->classes = o.recognizer_size == PPOCR_SIZE_TINY ? 6906 : 18710;
+    e->classes = ppocr::recognizer_classes(o.recognizer_size);
     if (e->classes != dictionary_len + 1 && e->classes != dictionary_len + 2)
       ppocr::raise(PPOCR_ERR_INVALID_INPUT, "recognizer has " + std::to_string(e->classes) +
                                                 " output classes, but the dictionary has " +
@@ -222,6 +230,22 @@ ppocr_status ppocr_hip_engine_load(ppocr_hip_ctx* ctx, const char* detector_path
 }
 
 void ppocr_hip_engine_free(ppocr_hip_engine* engine) { delete engine; }
+
+ppocr_status ppocr_hip_engine_set_rules(ppocr_hip_engine* e, const ppocr_class_rules* rules) {
+  return ppocr::guarded([&] {
+    if (!e) ppocr::raise(PPOCR_ERR_INVALID_INPUT, "engine is null");
+    const ppocr::ClassRules checked = ppocr::class_rules(rules, e->classes);
+    std::vector<float> bias;
+    std::vector<uint32_t> allowed;
+    if (checked.has_bias) bias.assign(rules->bias, rules->bias + e->classes);
+    if (checked.has_mask) allowed.assign(rules->allowed, rules->allowed + (e->classes + 31) / 32);
+    ppocr::sync_context(e->ctx);  // queued batches may still run the plans
+    e->shared_weights = nullptr;
+    e->recognizers.clear();
+    e->rule_bias.swap(bias);
+    e->rule_allowed.swap(allowed);
+  });
+}
 
 ppocr_status ppocr_hip_engine_recognize(ppocr_hip_engine* e, const uint8_t* rgb, uint32_t width, uint32_t height,
                                         ppocr_ocr_result** out) {

@@ -15,6 +15,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "logits.h"
 #include "runtime.h"
 
 namespace ppocr {
@@ -1062,6 +1063,63 @@ class Builder {
     add_op(std::move(op));
   }
 
+  // Rules of the tail on fp32 logits, in place.
+  void logit_rules(const View& x, const RecognizerTail& tail, const std::string& name) {
+    const View io = x;
+    Op op;
+    op.name = name;
+    op.kernel = "logit_rules";
+    op.bytes = 8.0 * x.pixels() * x.c;
+    op.reads = {x.buf};
+    op.writes = {x.buf};
+    op.launch = [=](const Exec& ex, hipStream_t s) {
+      launch_logit_rules(logit_rows(ex, io), tail_rules(ex, tail, io.c), ex.fptr(io), io.c, s);
+    };
+    add_op(std::move(op));
+  }
+
+  // The k best classes of each row of fp32 logits under the tail's rules and
+  // their probabilities, equal ones from the highest class down.
+  View top_classes(const View& x, const RecognizerTail& tail, int k, const std::string& name) {
+    View out = alloc(x.n, 1, x.w, 2 * k, "output", DT_F32);
+    const View in = x;
+    Op op;
+    op.name = name;
+    op.kernel = "top_logits";
+    op.bytes = 4.0 * x.pixels() * x.c + 8.0 * x.pixels() * k;
+    op.reads = {x.buf};
+    op.writes = {out.buf};
+    op.launch = [=](const Exec& ex, hipStream_t s) {
+      TopParams p{};
+      p.rules = tail_rules(ex, tail, in.c);
+      p.k = k;
+      p.temperature = 1.0f;
+      p.pairs = ex.fptr(out);
+      p.last_ties = 1;
+      launch_top_logits(logit_rows(ex, in), p, s);
+    };
+    add_op(std::move(op));
+    return out;
+  }
+
+  static LogitRows logit_rows(const Exec& ex, const View& x) {
+    return LogitRows{ex.ptr(x), (int64_t)x.pixels(), x.c, x.c, DT_F32};
+  }
+  static RuleParams tail_rules(const Exec& ex, const RecognizerTail& tail, int classes) {
+    RuleParams r{};
+    const char* at = ex.rules;
+    if (tail.has_bias) {
+      r.bias = reinterpret_cast<const float*>(at);
+      r.n_bias = 1;
+      at += (size_t)classes * sizeof(float);
+    }
+    if (tail.has_mask) {
+      r.masks = reinterpret_cast<const uint32_t*>(at);
+      r.n_masks = 1;
+    }
+    return r;
+  }
+
   // Classifier fused with the per-step half of greedy CTC decoding: for each
   // time step, the argmax class (ties -> last index) and its softmax
   // probability, the two values src/ocr.rs:800-853 takes from each row of
@@ -1719,6 +1777,12 @@ Plan build_detector(const SafeTensors& st, int size, const size_t nchw[4], int d
 // Recognizer::load (src/gpu/model.rs:156-220; architecture
 // src/cpu/model.rs:1961-2039).
 Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int dt, bool greedy) {
+  RecognizerTail tail;
+  tail.greedy = greedy;
+  return build_recognizer(st, size, nchw, dt, tail);
+}
+
+Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int dt, const RecognizerTail& tail) {
   validate_recognizer_shape(nchw);
   const size_t expected = size == PPOCR_SIZE_MEDIUM ? 269 : size == PPOCR_SIZE_SMALL ? 250 : 150;
   const char* tier = size == PPOCR_SIZE_MEDIUM ? "medium" : size == PPOCR_SIZE_SMALL ? "small" : "tiny";
@@ -1735,7 +1799,7 @@ Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int
   std::vector<View> stages = backbone(B, x, mid, out, !tiny, recognizer_stages(size));
   View pooled = B.avgpool32(stages.back(), "pool");
   if (pooled.h != 1) raise(PPOCR_ERR_INVALID_MODEL, "recognizer pooling must produce height 1");
-  const int classes = tiny ? 6906 : 18710;
+  const int classes = (int)recognizer_classes(size);
   View feat;  // classifier input [N, 1, T, C]
   ConvW cls;
   std::string cls_name;
@@ -1793,7 +1857,18 @@ Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int
     cls_name = "head.head";
   }
   const size_t n = (size_t)pooled.n, steps = (size_t)pooled.w;
-  if (greedy) {
+  const int top_k = tail.greedy && tail.ruled() ? 1 : tail.top_k;
+  if (top_k) {
+    View logits = B.alloc(pooled.n, 1, pooled.w, classes, "logits", DT_F32);
+    Epi into;
+    into.dst = &logits;
+    B.conv(feat, cls, into, cls_name);
+    View out = B.top_classes(logits, tail, top_k, "top");
+    plan.output = out.buf;
+    plan.output_elems = n * steps * top_k * 2;
+    plan.output_shape = {n, steps, 2};
+    if (!tail.greedy) plan.output_shape = {n, steps, (size_t)top_k, 2};
+  } else if (tail.greedy) {
     View out = B.greedy_classifier(feat, cls, cls_name);
     plan.output = out.buf;
     plan.output_elems = n * steps * 2;
@@ -1806,6 +1881,7 @@ Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int
     Epi into;
     into.dst = &logits;
     B.conv(feat, cls, into, cls_name);
+    if (tail.ruled()) B.logit_rules(logits, tail, "rules");
     B.softmax(logits, "softmax");
   }
   plan_arena(plan);

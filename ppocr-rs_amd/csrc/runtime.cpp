@@ -14,6 +14,7 @@
 
 #include <sys/mman.h>
 
+#include "logits.h"
 #include "runtime.h"
 
 namespace ppocr {
@@ -146,6 +147,7 @@ struct ppocr_hip_model {
   size_t item_in = 0, item_out = 0;  // fp32 input / output elements per item
   std::vector<size_t> out_shape;     // whole-batch output shape
   std::shared_ptr<ppocr::DeviceBuffer> weights;
+  std::shared_ptr<ppocr::DeviceBuffer> rules;  // class rules of a recognizer, or null
   size_t weight_blob_bytes = 0;
   std::string weights_path;
   int size = 0;
@@ -195,6 +197,7 @@ Exec exec_of(ppocr_hip_model* m) {
   ex.arena = m->ctx->arena;
   ex.weights = static_cast<const char*>(m->weights->ptr);
   ex.bufs = &m->plan.bufs;
+  ex.rules = m->rules ? static_cast<const char*>(m->rules->ptr) : nullptr;
   return ex;
 }
 
@@ -398,7 +401,9 @@ size_t largest_buffer(const Plan& plan) {
 
 ppocr_hip_model* load_model(ppocr_hip_ctx* ctx, const char* path, ppocr_model_size size, const size_t nchw[4],
                             ppocr_precision precision, const ppocr_hip_model* share, bool detector,
-                            bool greedy = false) {
+                            RecognizerTail tail = {}, const ClassRules& rules = {}) {
+  tail.has_bias = rules.has_bias;
+  tail.has_mask = rules.has_mask;
   if (!ctx) raise(PPOCR_ERR_INVALID_INPUT, "context is null");
   if (!path) raise(PPOCR_ERR_INVALID_INPUT, "weights path is null");
   if (!nchw) raise(PPOCR_ERR_INVALID_INPUT, "input shape is null");
@@ -412,7 +417,7 @@ ppocr_hip_model* load_model(ppocr_hip_ctx* ctx, const char* path, ppocr_model_si
   m->weights_path = path;
   std::copy(nchw, nchw + 4, m->in_shape);
   auto build = [&](const size_t* shape) {
-    return detector ? build_detector(st, size, shape, dt) : build_recognizer(st, size, shape, dt, greedy);
+    return detector ? build_detector(st, size, shape, dt) : build_recognizer(st, size, shape, dt, tail);
   };
   m->plan = build(nchw);
   m->chunk = nchw[0];
@@ -445,6 +450,11 @@ ppocr_hip_model* load_model(ppocr_hip_ctx* ctx, const char* path, ppocr_model_si
     HIP_OK(hipMemcpy(m->weights->ptr, m->plan.weights.data(), m->weight_blob_bytes, hipMemcpyHostToDevice));
   }
   std::vector<uint8_t>().swap(m->plan.weights);
+  if (rules.any()) {
+    const size_t bytes = rules.words.size() * sizeof(uint32_t);
+    m->rules = device_alloc(ctx->device, bytes);
+    HIP_OK(hipMemcpy(m->rules->ptr, rules.words.data(), bytes, hipMemcpyHostToDevice));
+  }
   ensure_arena(ctx, m->plan.arena_bytes);
   return m.release();
 }
@@ -525,7 +535,35 @@ ppocr_status ppocr_hip_recognizer_load_greedy(ppocr_hip_ctx* ctx, const char* pa
     *out = nullptr;
     if (share_weights && share_weights->plan.detector)
       raise(PPOCR_ERR_INVALID_INPUT, "shared weights must come from a recognizer");
-    *out = load_model(ctx, path, size, nchw, precision, share_weights, false, true);
+    RecognizerTail tail;
+    tail.greedy = true;
+    *out = load_model(ctx, path, size, nchw, precision, share_weights, false, tail);
+  });
+}
+
+ppocr_status ppocr_hip_recognizer_load_with(ppocr_hip_ctx* ctx, const char* path, ppocr_model_size size,
+                                            const size_t nchw[4], ppocr_precision precision,
+                                            const ppocr_recognizer_options* options,
+                                            const ppocr_hip_model* share_weights, ppocr_hip_model** out) {
+  return guarded([&] {
+    if (!out) raise(PPOCR_ERR_INVALID_INPUT, "output handle pointer is null");
+    *out = nullptr;
+    if (!options) raise(PPOCR_ERR_INVALID_INPUT, "options are null");
+    if (size < PPOCR_SIZE_MEDIUM || size > PPOCR_SIZE_TINY) raise(PPOCR_ERR_INVALID_INPUT, "unknown model size");
+    RecognizerTail tail;
+    tail.greedy = options->output == PPOCR_OUTPUT_GREEDY;
+    if (options->output < PPOCR_OUTPUT_PROBABILITIES || options->output > PPOCR_OUTPUT_TOP)
+      raise(PPOCR_ERR_INVALID_INPUT, "unknown recognizer output");
+    const bool top = options->output == PPOCR_OUTPUT_TOP;
+    if (top ? options->top_k == 0 || options->top_k > (size_t)kMaxTop : options->top_k != 0)
+      raise(PPOCR_ERR_INVALID_INPUT, "top_k must be 1 to " + std::to_string(kMaxTop) +
+                                         " for the best classes and 0 for other outputs, got " +
+                                         std::to_string(options->top_k));
+    tail.top_k = (int)options->top_k;
+    const ClassRules rules = class_rules(options->rules, recognizer_classes(size));
+    if (share_weights && share_weights->plan.detector)
+      raise(PPOCR_ERR_INVALID_INPUT, "shared weights must come from a recognizer");
+    *out = load_model(ctx, path, size, nchw, precision, share_weights, false, tail, rules);
   });
 }
 
@@ -734,6 +772,26 @@ void enqueue_forward_image(ppocr_hip_model* model, const ppocr_hip_image* image,
     run_image_graph(model);
     queue_download(model, out, c);
   }
+}
+
+ClassRules class_rules(const ppocr_class_rules* rules, size_t classes) {
+  ClassRules r;
+  if (!rules) return r;
+  if (rules->classes != classes)
+    raise(PPOCR_ERR_INVALID_INPUT, "class rules for " + std::to_string(rules->classes) + " classes; the recognizer has " +
+                                       std::to_string(classes));
+  if (rules->bias) {
+    if (!all_finite(rules->bias, classes)) raise(PPOCR_ERR_INVALID_INPUT, "class biases contain non-finite values");
+    r.has_bias = true;
+    r.words.resize(classes);
+    memcpy(r.words.data(), rules->bias, classes * sizeof(float));
+  }
+  if (rules->allowed) {
+    if (!(rules->allowed[0] & 1)) raise(PPOCR_ERR_INVALID_INPUT, "the blank (class 0) must be allowed");
+    r.has_mask = true;
+    r.words.insert(r.words.end(), rules->allowed, rules->allowed + (classes + 31) / 32);
+  }
+  return r;
 }
 
 int context_device(const ppocr_hip_ctx* ctx) { return ctx->device; }

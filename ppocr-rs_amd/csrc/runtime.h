@@ -108,6 +108,7 @@ struct Exec {
   char* arena = nullptr;
   const char* weights = nullptr;
   const std::vector<Buffer>* bufs = nullptr;
+  const char* rules = nullptr;  // a recognizer's class rules (ClassRules layout)
   void* ptr(const View& v) const { return arena + (*bufs)[v.buf].arena_off + v.off * dtype_size(v.dt); }
   float* fptr(const View& v) const { return static_cast<float*>(ptr(v)); }
   // Weight blob offsets are in bytes; SIZE_MAX means "absent".
@@ -144,6 +145,27 @@ struct Plan {
   int dt = DT_F32;  // activation storage type
 };
 
+// Rules on a recognizer's classes as the device holds them: the biases (when
+// has_bias), then the words of the allowed classes (when has_mask).
+struct ClassRules {
+  bool has_bias = false, has_mask = false;
+  std::vector<uint32_t> words;
+  bool any() const { return has_bias || has_mask; }
+};
+// Checked copy of the rules of a recognizer of `classes` classes.
+ClassRules class_rules(const ppocr_class_rules* rules, size_t classes);
+// Classes of a recognizer tier.
+inline size_t recognizer_classes(int size) { return size == PPOCR_SIZE_TINY ? 6906 : 18710; }
+
+// What a recognizer's plan ends in besides greedy decoding without rules and
+// plain probabilities: the top_k best classes of each step (0: none), rules.
+struct RecognizerTail {
+  bool greedy = false;
+  int top_k = 0;
+  bool has_bias = false, has_mask = false;
+  bool ruled() const { return has_bias || has_mask; }
+};
+
 // Builds the plan of one model for a fixed input shape; `dt` selects fp32 or
 // bf16 activation storage.  A `greedy` recognizer ends in the classifier
 // fused with per-step greedy CTC decoding (output [N, T, 2]: class index,
@@ -151,6 +173,9 @@ struct Plan {
 // pack the same weight blob.
 Plan build_detector(const SafeTensors& st, int size, const size_t nchw[4], int dt);
 Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int dt, bool greedy);
+// With rules, or with the top_k best classes [N, T, k, 2], the classifier's
+// logits are stored and the operators on rows of logits take them from there.
+Plan build_recognizer(const SafeTensors& st, int size, const size_t nchw[4], int dt, const RecognizerTail& tail);
 
 // Every point where a plan rounds to its bf16 storage type, in op order:
 // "A <value>" for each activation value rounded (a bf16 buffer's name when

@@ -43,7 +43,7 @@ EXPORTS = (
     "ppocr_hip_engine_load", "ppocr_hip_engine_free", "ppocr_hip_engine_recognize", "ppocr_ocr_result_lines",
     "ppocr_ocr_result_tokens", "ppocr_ocr_result_sizes", "ppocr_ocr_result_free",
     "ppocr_hip_logit_rules", "ppocr_hip_top_logits", "ppocr_hip_distill_loss", "ppocr_hip_distill_grad",
-    "ppocr_hip_distill",
+    "ppocr_hip_distill", "ppocr_hip_recognizer_load_with", "ppocr_hip_engine_set_rules",
 )
 
 
@@ -157,6 +157,18 @@ class _Rules(ctypes.Structure):
                 ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p)]
 
 
+class _ClassRules(ctypes.Structure):
+    """``ppocr_class_rules``."""
+
+    _fields_ = [("classes", ctypes.c_size_t), ("bias", ctypes.c_void_p), ("allowed", ctypes.c_void_p)]
+
+
+class _RecognizerOptions(ctypes.Structure):
+    """``ppocr_recognizer_options``."""
+
+    _fields_ = [("output", ctypes.c_int), ("top_k", ctypes.c_size_t), ("rules", ctypes.POINTER(_ClassRules))]
+
+
 class _Teacher(ctypes.Structure):
     """``ppocr_teacher``."""
 
@@ -225,6 +237,9 @@ def lib():
         L.ppocr_hip_distill_loss.argtypes = [_VP, _LG, _TE, ctypes.c_float, _VP, _VP, _VP]
         L.ppocr_hip_distill_grad.argtypes = [_VP, _LG, _TE, _VP, ctypes.c_float, _VP, _VP, ctypes.c_size_t, _VP]
         L.ppocr_hip_distill.argtypes = [_VP, _LG, _TE, ctypes.c_float, _VP, _VP, _VP, ctypes.c_size_t, _VP]
+        L.ppocr_hip_recognizer_load_with.argtypes = [_VP, ctypes.c_char_p, ctypes.c_int, _SZ, ctypes.c_int,
+                                                     ctypes.POINTER(_RecognizerOptions), _VP, ctypes.POINTER(_VP)]
+        L.ppocr_hip_engine_set_rules.argtypes = [_VP, ctypes.POINTER(_ClassRules)]
         _lib = L
     return _lib
 
@@ -658,15 +673,47 @@ class Detector(_Model):
             o.max_boxes)
 
 
+def _class_rules(classes, allowed, bias):
+    """``ppocr_class_rules`` and the arrays that it points to."""
+    rules = _ClassRules(classes=classes)
+    if bias is not None:
+        bias = np.ascontiguousarray(bias, dtype=np.float32)
+        if bias.shape != (classes,):
+            raise ValueError(f"bias needs {classes} values")
+        rules.bias = bias.ctypes.data
+    if allowed is not None:
+        allowed = np.asarray(allowed, dtype=bool)
+        if allowed.shape != (classes,):
+            raise ValueError(f"allowed needs {classes} values")
+        bits = np.zeros(-(-classes // 32) * 32, bool)
+        bits[:classes] = allowed
+        allowed = np.packbits(bits, bitorder="little").view("<u4")
+        rules.allowed = allowed.ctypes.data
+    return rules, (bias, allowed)
+
+
 class Recognizer(_Model):
     """``gpu::Recognizer`` (src/gpu/model.rs:150-266)."""
 
     @classmethod
-    def load(cls, gpu, path, size, input_shape, precision="f32", share_weights=None, greedy=False):
+    def load(cls, gpu, path, size, input_shape, precision="f32", share_weights=None, greedy=False, top_k=0,
+             allowed=None, bias=None):
         """``Recognizer::load`` / ``load_with_shared_weights``.  With ``greedy``
         the classifier is fused with per-step greedy CTC decoding and the
-        output is [N, T, 2] (class index, probability) per time step."""
+        output is [N, T, 2] (class index, probability) per time step; with
+        ``top_k`` it is [N, T, top_k, 2], the best classes of each step.
+        ``allowed`` [classes] (booleans) and ``bias`` [classes] are rules on the
+        classes."""
         h = _VP()
+        if top_k or allowed is not None or bias is not None:
+            if greedy and top_k:
+                raise ValueError("greedy and top_k are two outputs")
+            rules, _kept = _class_rules(6906 if size == "tiny" else 18710, allowed, bias)
+            options = _RecognizerOptions(1 if greedy else 2 if top_k else 0, int(top_k), ctypes.pointer(rules))
+            _check(lib().ppocr_hip_recognizer_load_with(
+                gpu.handle, str(path).encode(), SIZE_CODE[size], _sizes(input_shape), PRECISION[precision],
+                ctypes.byref(options), share_weights.handle if share_weights is not None else None, ctypes.byref(h)))
+            return cls(gpu, h, input_shape)
         entry = lib().ppocr_hip_recognizer_load_greedy if greedy else lib().ppocr_hip_recognizer_load
         _check(entry(gpu.handle, str(path).encode(), SIZE_CODE[size], _sizes(input_shape), PRECISION[precision],
                      share_weights.handle if share_weights is not None else None, ctypes.byref(h)))
@@ -806,6 +853,14 @@ class OcrEngine:
         _check(L.ppocr_hip_engine_load(gpu.handle, str(detector_model).encode(), str(recognizer_model).encode(),
                                        len(dictionary), ctypes.byref(o), ctypes.byref(h)))
         return cls(gpu, h, dictionary, 6906 if recognizer_size == "tiny" else 18710)
+
+    def set_rules(self, allowed=None, bias=None):
+        """Rules on the classes of every line from here on: ``allowed``
+        [classes] (booleans, the blank among them) and ``bias`` [classes];
+        neither: none."""
+        rules, _kept = _class_rules(self.classes, allowed, bias)
+        none = allowed is None and bias is None
+        _check(_engine_lib().ppocr_hip_engine_set_rules(self.handle, None if none else ctypes.byref(rules)))
 
     def recognize(self, rgb):
         """``OcrEngine::recognize`` (src/ocr.rs:497-522) on an HxWx3 uint8 image."""
