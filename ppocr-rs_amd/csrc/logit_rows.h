@@ -118,6 +118,14 @@ struct PackRegs {
   __device__ __forceinline__ void load(const T* p) { Pack<T>::load(p, v); }
   __device__ __forceinline__ float get(int e) const { return v[e]; }
   __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
+  // Elements whose bit is 0 become -inf: a bit stretched over the word selects.
+  __device__ __forceinline__ void keep(unsigned bits) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const uint32_t m = (uint32_t)((int)(bits << (31 - e)) >> 31);
+      v[e] = __uint_as_float((__float_as_uint(v[e]) & m) | (0xFF800000u & ~m));
+    }
+  }
   __device__ __forceinline__ void clear(int e) { v[e] = -INFINITY; }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -184,13 +192,15 @@ struct RowShape {
   }
 };
 
-// Reads part `seg`; classes past the row are -inf.
+// Reads part `seg`; classes past the row are -inf, and so are packs without a
+// bit in `bits` (PER of them, or null), which are not read.
 template <typename P, typename T, int N>
-__device__ __forceinline__ void load_part(P& d, const T* x, const RowShape<N>& s, int seg) {
+__device__ __forceinline__ void load_part(P& d, const T* x, const RowShape<N>& s, int seg,
+                                          const unsigned* bits = nullptr) {
 #pragma unroll
   for (int j = 0; j < P::kPer; ++j) {
     const int i = (seg * P::kPer + j) * P::kThreads + (int)threadIdx.x;
-    if (i < s.full)
+    if (bits ? bits[j] != 0 : i < s.full)
       d.pack[j].load(x + s.pack_class(i));
     else
       d.pack[j].clear();

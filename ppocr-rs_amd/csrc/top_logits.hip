@@ -33,73 +33,78 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* red) {
   return r;
 }
 
-// The rules on a part in registers.  The history is counted in windows of
+// The rules of a launch: none, biases and masks, or penalties too (whose
+// counting costs registers).
+enum RuleParts { kNoRules, kTables, kHistory };
+
+// The penalties on a part in registers.  The history is counted in windows of
 // kWindow classes, whole rounds of packs; the row's last classes have counters
 // of their own behind the window's.
 constexpr int kWindow = 8192;
 
 template <typename P, int N>
-__device__ __forceinline__ void rule_part(P& d, const RowRules& r, const RowShape<N>& s, int seg, int* counts) {
+__device__ __forceinline__ void penalise_part(P& d, const RowRules& r, const RowShape<N>& s, int seg, int* counts) {
   constexpr int NT = P::kThreads, PER = P::kPer, kRounds = kWindow / (NT * N);
   static_assert(kRounds >= 1 && kWindow % (NT * N) == 0, "a window is whole rounds");
-  const int tail = s.tail_class();
-  if (r.n_history) {
-    if (seg == 0 && s.full * N < s.classes) {
-      __syncthreads();
-      count_history(r, s.full * N, s.classes - s.full * N, counts + kWindow);
-      if (tail < s.classes && counts[kWindow + threadIdx.x] > 0)
-        d.tail = penalise(r, d.tail, counts[kWindow + threadIdx.x]);
-    }
+  if (seg == 0 && s.full * N < s.classes) {
+    __syncthreads();
+    count_history(r, s.full * N, s.classes - s.full * N, counts + kWindow);
+    if (s.has_tail() && counts[kWindow + threadIdx.x] > 0) d.tail = penalise(r, d.tail, counts[kWindow + threadIdx.x]);
+  }
 #pragma unroll
-    for (int w = 0; w < PER; w += kRounds) {
-      const int i0 = (seg * PER + w) * NT, i1 = min(i0 + kRounds * NT, s.full);
-      if (i0 < s.full) {
-        const int first = min(s.pack_class(i0), s.pack_class(i1 - 1));
-        __syncthreads();  // the window before is no longer read
-        count_history(r, first, (i1 - i0) * N, counts);
+  for (int w = 0; w < PER; w += kRounds) {
+    const int i0 = (seg * PER + w) * NT, i1 = min(i0 + kRounds * NT, s.full);
+    if (i0 < s.full) {
+      const int first = min(s.pack_class(i0), s.pack_class(i1 - 1));
+      __syncthreads();  // the window before is no longer read
+      count_history(r, first, (i1 - i0) * N, counts);
 #pragma unroll
-        for (int j = w; j < w + kRounds && j < PER; ++j) {
-          const int i = (seg * PER + j) * NT + (int)threadIdx.x;
-          if (i < s.full)
+      for (int j = w; j < w + kRounds && j < PER; ++j) {
+        const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+        if (i < s.full)
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-              const int c = counts[s.pack_class(i) - first + e];
-              if (c > 0) d.pack[j].set(e, penalise(r, d.pack[j].get(e), c));
-            }
-        }
+          for (int e = 0; e < N; ++e) {
+            const int c = counts[s.pack_class(i) - first + e];
+            if (c > 0) d.pack[j].set(e, penalise(r, d.pack[j].get(e), c));
+          }
       }
     }
-  }
-  if (r.bias) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int i = (seg * PER + j) * NT + (int)threadIdx.x;
-      if (i < s.full) {
-        float b[N];
-        load_bias<N>(r.bias + s.pack_class(i), b);
-#pragma unroll
-        for (int e = 0; e < N; ++e) d.pack[j].set(e, d.pack[j].get(e) + b[e]);
-      }
-    }
-    if (seg == 0 && tail < s.classes) d.tail = d.tail + r.bias[tail];
-  }
-  if (r.mask) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int i = (seg * PER + j) * NT + (int)threadIdx.x;
-      const unsigned bits = i < s.full ? mask_bits<N>(r.mask, s.pack_class(i)) : 0;
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (!(bits >> e & 1)) d.pack[j].clear(e);
-    }
-    if (seg == 0 && tail < s.classes && !mask_bit(r.mask, tail)) d.tail = -INFINITY;
   }
 }
 
-template <bool RULES, typename P, typename T, int N>
+// Reads a part under the rules.  Packs without an allowed class are not read.
+template <RuleParts RULES, typename P, typename T, int N>
 __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, const RowShape<N>& s, int seg, int* counts) {
-  load_part(d, x, s, seg);
-  if constexpr (RULES) rule_part(d, r, s, seg, counts);
+  constexpr int NT = P::kThreads, PER = P::kPer;
+  if constexpr (RULES == kNoRules) {
+    load_part(d, x, s, seg);
+  } else {
+    unsigned bits[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+      bits[j] = i < s.full ? (r.mask ? mask_bits<N>(r.mask, s.pack_class(i)) : (1u << N) - 1) : 0;
+    }
+    load_part(d, x, s, seg, bits);
+    if constexpr (RULES == kHistory)
+      if (r.n_history) penalise_part(d, r, s, seg, counts);
+    if (r.bias) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (bits[j]) {
+          float b[N];
+          load_bias<N>(r.bias + s.pack_class((seg * PER + j) * NT + (int)threadIdx.x), b);
+#pragma unroll
+          for (int e = 0; e < N; ++e) d.pack[j].set(e, d.pack[j].get(e) + b[e]);
+        }
+      if (seg == 0 && s.has_tail()) d.tail = d.tail + r.bias[s.tail_class()];
+    }
+    if (r.mask) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) d.pack[j].keep(bits[j]);
+      if (seg == 0 && s.has_tail() && !mask_bit(r.mask, s.tail_class())) d.tail = -INFINITY;
+    }
+  }
 }
 
 // The k best classes of a row and the log-sum-exp of the others, one row a
@@ -177,14 +182,14 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
 
 // The slow way for any row: k searches for the best class below the last one,
 // then the sums of the others, the row read each time.
-template <typename T, bool RULES, int W>
+template <typename T, RuleParts RULES, int W>
 __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int classes, const TopParams& p, float c,
                                            int* counts, TopShared<W>& sh, float& wm, double& ws) {
   const auto each = [&](auto&& f) {
     for (int first = 0; first < classes; first += kWindow) {
       const int n = min(kWindow, classes - first);
       bool counted = false;
-      if constexpr (RULES) {
+      if constexpr (RULES == kHistory) {
         counted = r.n_history > 0;
         if (counted) {
           __syncthreads();
@@ -193,7 +198,7 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
       }
       for (int i = threadIdx.x; i < n; i += blockDim.x) {
         float v = ld1<T>(x + first + i);
-        if constexpr (RULES) v = apply_rules(r, v, first + i, counted ? counts[i] : 0);
+        if constexpr (RULES != kNoRules) v = apply_rules(r, v, first + i, counted ? counts[i] : 0);
         f(v, order_key(v, first + i, p.last_ties));
       }
     }
@@ -220,13 +225,15 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
 }
 
 // Waves a SIMD that the registers of a part leave room for.
-template <typename T, int NT, int PER, bool RULES>
+template <typename T, int NT, int PER, RuleParts RULES>
 constexpr int top_waves() {
-  constexpr int regs = RULES ? PER * Pack<T>::N : PER * 4;
-  return NT == 1024 ? 4 : regs <= 32 ? RULES ? 5 : 7 : regs <= 40 ? 5 : RULES ? 3 : 4;
+  constexpr int regs = RULES != kNoRules ? PER * Pack<T>::N : PER * 4;
+  if (NT == 1024 || (RULES == kNoRules && regs > 40)) return 4;
+  if (RULES != kNoRules) return regs <= 40 ? 5 : 3;
+  return regs <= 32 ? 7 : 5;
 }
 
-template <typename T, int NT, int PER, bool RULES>
+template <typename T, int NT, int PER, RuleParts RULES>
 __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logits_kernel(LogitRows in, TopParams p, int parts) {
   constexpr int N = Pack<T>::N, W = NT / 64;
   __shared__ TopShared<W> sh;
@@ -235,13 +242,13 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(in.x) + row * in.stride;
   RowRules r{};
-  if constexpr (RULES) r = row_rules(p.rules, row, in.classes);
+  if constexpr (RULES != kNoRules) r = row_rules(p.rules, row, in.classes);
   const RowShape<N> shape(in.classes, p.last_ties);
   const float c = kLog2e / p.temperature;
   if (tid == 0) sh.nan = 0;
 
   // Best logit of this thread and the first place that holds it.
-  RowPart<T, NT, PER, !RULES> d;
+  RowPart<T, NT, PER, RULES == kNoRules> d;
   float high[PER];  // each pack's maximum
   float best = -INFINITY;
   int place = 0;
@@ -381,18 +388,22 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   }
 }
 
-template <typename T, int NT, int PER, bool RULES>
+template <typename T, int NT, int PER, RuleParts RULES>
 void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int kClasses = NT * PER * Pack<T>::N;
-  const size_t lds = p.rules.history ? (kWindow + 8) * sizeof(int) : 0;
+  const size_t lds = RULES == kHistory ? (kWindow + 8) * sizeof(int) : 0;
   hipLaunchKernelGGL((top_logits_kernel<T, NT, PER, RULES>), dim3((unsigned)in.rows), dim3(NT), lds, s, in, p,
                      (in.classes + kClasses - 1) / kClasses);
 }
 
-// Threads of a row's workgroup and the elements that each holds.
-template <typename T, bool RULES>
-void launch_top_typed(const LogitRows& in, const TopParams& p, hipStream_t s) {
-  constexpr int N = Pack<T>::N, kLong = RULES ? 64 : 80;
+// Threads of a row's workgroup and the elements that each holds.  A few hundred
+// rows fill the chip better with 512 threads (378 x 18710 fp32 under masks, top
+// 3: 14.5 us against 20.4 with 1024 and 20.8 with 256), batches with 256, whose
+// waves share the work of bound and ranking (10240 x 18710 fp32, top 64: 149 us
+// against 223 with 512).
+template <typename T, RuleParts RULES>
+void launch_top_rules(const LogitRows& in, const TopParams& p, hipStream_t s) {
+  constexpr int N = Pack<T>::N, kLong = RULES != kNoRules ? 64 : 80;
   if (in.rows < 1024 && in.classes > 256 * 8 && in.classes <= 512 * 40)
     launch_top<T, 512, 40 / N, RULES>(in, p, s);
   else if (in.classes <= 256 * 32)
@@ -403,13 +414,20 @@ void launch_top_typed(const LogitRows& in, const TopParams& p, hipStream_t s) {
     launch_top<T, 1024, kLong / N, RULES>(in, p, s);
 }
 
+template <typename T>
+void launch_top_typed(const LogitRows& in, const TopParams& p, hipStream_t s) {
+  if (p.rules.history)
+    launch_top_rules<T, kHistory>(in, p, s);
+  else if (p.rules.bias || p.rules.masks)
+    launch_top_rules<T, kTables>(in, p, s);
+  else
+    launch_top_rules<T, kNoRules>(in, p, s);
+}
+
 }  // namespace
 
 void launch_top_logits(const LogitRows& in, const TopParams& p, hipStream_t s) {
-  if (p.rules.history || p.rules.bias || p.rules.masks)
-    in.dt == DT_BF16 ? launch_top_typed<bf16, true>(in, p, s) : launch_top_typed<float, true>(in, p, s);
-  else
-    in.dt == DT_BF16 ? launch_top_typed<bf16, false>(in, p, s) : launch_top_typed<float, false>(in, p, s);
+  in.dt == DT_BF16 ? launch_top_typed<bf16>(in, p, s) : launch_top_typed<float>(in, p, s);
 }
 
 }  // namespace ppocr
