@@ -230,7 +230,7 @@ constexpr int top_waves() {
   constexpr int regs = RULES != kNoRules ? PER * Pack<T>::N : PER * 4;
   if (NT == 1024 || (RULES == kNoRules && regs > 40)) return 4;
   if (RULES != kNoRules) return regs <= 40 ? 5 : 3;
-  return regs <= 32 ? 7 : 5;
+  return regs <= 32 ? 7 : 4;
 }
 
 template <typename T, int NT, int PER, RuleParts RULES>
