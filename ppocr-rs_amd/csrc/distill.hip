@@ -56,11 +56,11 @@ constexpr int distill_waves() {
 // is a difference of logs that nearly cancel.  An entry that does not count
 // loses its index.
 __device__ __forceinline__ void teacher_shares(const DistillParams& p, int64_t row, TeacherEntry& entry, double inv,
-                                               DistillShared& sh) {
+                                               bool maybe_again, DistillShared& sh) {
   const int lane = threadIdx.x & 63;
   // A class named twice counts once, with its first entry.
   bool again = false;
-  for (int j = 0; j + 1 < p.k; ++j) again |= __builtin_amdgcn_readlane(entry.index, j) == entry.index && j < lane;
+  for (int j = 0; maybe_again && j + 1 < p.k; ++j) again |= __builtin_amdgcn_readlane(entry.index, j) == entry.index && j < lane;
   if (again) entry.index = -1;
   const bool valid = entry.index >= 0;
   const double rest = p.rest ? (double)p.rest[row] : -INFINITY;
@@ -112,11 +112,15 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
 #pragma unroll
       for (int i = 0; i < kWords; ++i) marks[tid * kWords + i] = 0;
       __syncthreads();
+      bool again = PARTS;  // whether a class may be named twice: its mark was set already
       if (wave == 0 && entry.index >= 0) {
         const int i = entry.index / N, at = i - seg * PER * NT;
-        if (i < shape.full && at >= 0 && at < PER * NT) {
+        if (i >= shape.full) {
+          again = true;  // the row's last classes have no marks
+        } else if (at >= 0 && at < PER * NT) {
           const int j = at / NT;
-          atomicOr(&marks[(at - j * NT) * kWords + (j >> 2)], 1u << ((j & 3) * 8 + entry.index % N));
+          const uint32_t bit = 1u << ((j & 3) * 8 + entry.index % N);
+          again = (atomicOr(&marks[(at - j * NT) * kWords + (j >> 2)], bit) & bit) != 0;
         }
       }
       __syncthreads();
@@ -135,7 +139,7 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
         for (int j = 0; j < p.k; ++j)
           if (__builtin_amdgcn_readlane(entry.index, j) == shape.tail_class()) d.tail = -INFINITY;
       }
-      if (seg == 0 && wave == 0) teacher_shares(p, row, entry, inv, sh);
+      if (seg == 0 && wave == 0) teacher_shares(p, row, entry, inv, lanes_where(again) != 0, sh);
       float pm = part_max(d);
       const double ps = part_sum(d, fmaxf(pm, -FLT_MAX), c);
       if (ps != ps) pm = fmaxf(pm, -FLT_MAX);  // a NaN is no maximum but must not be lost
@@ -148,7 +152,7 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
 
   float entry_grad = 0.0f;
   if (wave == 0) {
-    if constexpr (MODE == kGradient) teacher_shares(p, row, entry, inv, sh);
+    if constexpr (MODE == kGradient) teacher_shares(p, row, entry, inv, true, sh);
     const bool valid = entry.index >= 0;
     const double q = sh.q[lane], q0 = sh.q0;
     double top, z, mr, zr;
