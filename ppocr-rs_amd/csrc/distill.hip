@@ -28,8 +28,7 @@ __device__ __forceinline__ TeacherEntry teacher_entry(const DistillParams& p, in
 //   loss = tau^2 (sum_j q_j (log q_j - log p_j) + q0 (log q0 - log p0)),
 //   d loss / d s_c = tau (p_c - q_c) for an entry, tau e_c (1 / Z - q0 / Z0) else.
 // So the rest's gradient is e times one factor of the row, and the row is read
-// once: it stays in registers with the entries taken out (their marks come
-// through LDS, a byte a pack).  Wave 0 does the entries, in 64 bits, the
+// once: it stays in registers with the entries taken out (by marks in LDS).  Wave 0 does the entries, in 64 bits, the
 // teacher's shares while the row is on its way, and writes their gradients over
 // the row's.  The whole is formed from the rest and the entries, so that the
 // shares add up to one and an error of the rest's sum cancels to first order in
@@ -46,10 +45,9 @@ struct DistillShared {
 };
 
 // Waves a SIMD that the registers of a part leave room for.
-template <typename T, int NT, int PER, bool PARTS>
+template <int PER>
 constexpr int distill_waves() {
-  constexpr int regs = PER * 4;
-  return NT == 1024 && PARTS ? 4 : regs <= 16 ? 8 : regs <= 40 ? 5 : 4;
+  return PER * 4 <= 16 ? 8 : 5;
 }
 
 // The teacher's shares of a row and their logs, by wave 0, in 64 bits: the loss
@@ -73,12 +71,71 @@ __device__ __forceinline__ void teacher_shares(const DistillParams& p, int64_t r
   if (lane == 0) sh.q0 = x0 / sum, sh.logq0 = rest - m - logsum;
 }
 
+// Marks of the entries' classes below the row's last classes % N: a bit a class,
+// for all parts of a row at once, so that the waves run through the parts
+// without waiting for each other (256 x 131072 fp32, loss: 29.4 us against 44
+// with marks by the part).  An fp32 row of one part has a byte a pack instead, a
+// thread's bytes together, so that a thread reads four packs' marks at once
+// (10240 x 18710, loss: 126 us against 144); in bf16, with half as many packs,
+// bits are faster (92 us against 98).
+template <int N, int NT, int PER, bool PARTS>
+struct Marks {
+  static constexpr bool kBits = PARTS || N == 8;
+  static constexpr int kWords = (PER + 3) / 4;
+  const RowShape<N>& shape;
+  uint32_t* at;
+
+  static size_t words(int classes) { return kBits ? (size_t)(classes + 31) / 32 : (size_t)NT * kWords; }
+  __device__ __forceinline__ void reset() {
+    if constexpr (kBits) {
+      for (int i = threadIdx.x; i < (shape.classes + 31) / 32; i += NT) at[i] = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) at[threadIdx.x * kWords + i] = 0;
+    }
+  }
+  // Marks a class; whether it may have been marked before.
+  __device__ __forceinline__ bool set(int c) {
+    const int i = c / N;
+    if (i >= shape.full) return true;
+    const int word = kBits ? c >> 5 : i % NT * kWords + (i / NT >> 2);
+    const uint32_t bit = 1u << (kBits ? c & 31 : (i / NT & 3) * 8 + c % N);
+    return (atomicOr(&at[word], bit) & bit) != 0;
+  }
+  // Takes the marked classes out of a part.
+  template <typename P>
+  __device__ __forceinline__ void clear(P& d, int seg) const {
+    if constexpr (kBits) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = (seg * PER + j) * NT + (int)threadIdx.x;
+        const unsigned bits = i < shape.full ? mask_bits<N>(at, i * N) : 0;
+        if (bits)
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (bits >> e & 1) d.pack[j].clear(e);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const uint32_t word = at[threadIdx.x * kWords + w];
+        if (word)
+#pragma unroll
+          for (int q = 0; q < 4 && w * 4 + q < PER; ++q)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (word >> (q * 8 + e) & 1) d.pack[w * 4 + q].clear(e);
+      }
+    }
+  }
+};
+
 // PARTS: rows of `parts` parts; else the whole row is one.
 template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
-__global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void distill_kernel(LogitRows s, DistillParams p, int parts) {
-  constexpr int N = Pack<T>::N, W = NT / 64, kWords = (PER + 3) / 4;
+__global__ __launch_bounds__(NT, distill_waves<PER>()) void distill_kernel(LogitRows s, DistillParams p, int parts) {
+  constexpr int N = Pack<T>::N, W = NT / 64;
   __shared__ DistillShared sh;
-  __shared__ uint32_t marks[MODE == kGradient ? 1 : NT * kWords];
+  extern __shared__ uint32_t mark_words[];  // not of the gradient alone
   const int segs = PARTS ? parts : 1;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
@@ -107,44 +164,25 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
   double sum = 0.0;
   if (!PARTS || MODE != kGradient) load_part(d, x, shape, 0);
   if constexpr (MODE != kGradient) {
+    Marks<N, NT, PER, PARTS> marks{shape, mark_words};
+    marks.reset();
+    __syncthreads();
+    bool again = false;  // whether a class may be named twice
+    if (wave == 0 && entry.index >= 0) again = marks.set(entry.index);
+    __syncthreads();
+    if (wave == 0) teacher_shares(p, row, entry, inv, lanes_where(again) != 0, sh);
     for (int seg = 0; seg < segs; ++seg) {
       if (seg > 0) load_part(d, x, shape, seg);
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) marks[tid * kWords + i] = 0;
-      __syncthreads();
-      bool again = PARTS;  // whether a class may be named twice: its mark was set already
-      if (wave == 0 && entry.index >= 0) {
-        const int i = entry.index / N, at = i - seg * PER * NT;
-        if (i >= shape.full) {
-          again = true;  // the row's last classes have no marks
-        } else if (at >= 0 && at < PER * NT) {
-          const int j = at / NT;
-          const uint32_t bit = 1u << ((j & 3) * 8 + entry.index % N);
-          again = (atomicOr(&marks[(at - j * NT) * kWords + (j >> 2)], bit) & bit) != 0;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        const uint32_t word = marks[tid * kWords + w];
-        if (word)
-#pragma unroll
-          for (int q = 0; q < 4 && w * 4 + q < PER; ++q)
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (word >> (q * 8 + e) & 1) d.pack[w * 4 + q].clear(e);
-      }
-      if (seg == 0 && 0 != lanes_where(entry.index >= shape.full * N)) {
+      marks.clear(d, seg);
+      if (seg == 0 && lanes_where(entry.index >= shape.full * N)) {
         // Entries among the row's last classes, one a thread.
         for (int j = 0; j < p.k; ++j)
           if (__builtin_amdgcn_readlane(entry.index, j) == shape.tail_class()) d.tail = -INFINITY;
       }
-      if (seg == 0 && wave == 0) teacher_shares(p, row, entry, inv, lanes_where(again) != 0, sh);
       float pm = part_max(d);
       const double ps = part_sum(d, fmaxf(pm, -FLT_MAX), c);
       if (ps != ps) pm = fmaxf(pm, -FLT_MAX);  // a NaN is no maximum but must not be lost
       join_sums(m, sum, pm, ps, c);
-      if (PARTS) __syncthreads();  // the marks are no longer read
     }
     if (lane == 0) sh.max[wave] = m, sh.sum[wave] = sum;
     __syncthreads();
@@ -226,28 +264,29 @@ __global__ __launch_bounds__(NT, (distill_waves<T, NT, PER, PARTS>())) void dist
 template <typename T, int NT, int PER, bool PARTS, DistillMode MODE>
 void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t s) {
   constexpr int kClasses = NT * PER * Pack<T>::N;
-  hipLaunchKernelGGL((distill_kernel<T, NT, PER, PARTS, MODE>), dim3((unsigned)in.rows), dim3(NT), 0, s, in, p,
+  const size_t lds = MODE == kGradient ? 0 : Marks<Pack<T>::N, NT, PER, PARTS>::words(in.classes) * sizeof(uint32_t);
+  hipLaunchKernelGGL((distill_kernel<T, NT, PER, PARTS, MODE>), dim3((unsigned)in.rows), dim3(NT), lds, s, in, p,
                      (in.classes + kClasses - 1) / kClasses);
 }
 
 // Threads of a row's workgroup and the elements that each holds.  512 threads
 // of 40 elements keep more waves on a CU than 256 of 80 (2560 x 18710 fp32, loss
-// and gradient: 80 us against 105); the loss alone needs so few registers that
-// batches are even in fp32 and faster with 256 in bf16 (10240 x 18710: 98 us
-// against 109), but a few hundred rows fill the chip better with 512 (378 x
-// 18710 fp32: 9.3 us against 12.4).
+// and gradient: 80 us against 105), but for the loss alone of bf16 batches,
+// whose rows take half the registers (10240 x 18710: 92 us against 109).
 template <typename T, DistillMode MODE>
 void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N;
-  const bool wide = in.rows < 1024 || (MODE != kLoss && in.classes > 256 * 32);
-  if (wide && in.classes > 256 * 8 && in.classes <= 512 * 40)
-    launch_distill_one<T, 512, 40 / N, false, MODE>(in, p, s);
-  else if (in.classes <= 256 * 32)
+  constexpr bool kSlim = MODE == kLoss && sizeof(T) == 2;
+  if (in.classes <= 256 * 8 || (in.rows >= 1024 && in.classes <= 256 * 32))
     launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
-  else if (MODE == kLoss && in.classes <= 256 * 80)
-    launch_distill_one<T, 256, 80 / N, false, kLoss>(in, p, s);
+  else if (kSlim && in.rows >= 1024 && in.classes <= 256 * 80)
+    launch_distill_one<bf16, 256, 80 / 8, false, kLoss>(in, p, s);
+  else if (in.classes <= 512 * 40)
+    launch_distill_one<T, 512, 40 / N, false, MODE>(in, p, s);
+  else if (in.classes <= 1024 * 40)
+    launch_distill_one<T, 1024, 40 / N, false, MODE>(in, p, s);
   else
-    launch_distill_one<T, 1024, 80 / N, true, MODE>(in, p, s);
+    launch_distill_one<T, 1024, 40 / N, true, MODE>(in, p, s);
 }
 
 template <DistillMode MODE>

@@ -31,7 +31,6 @@ __global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, Rul
     const int i = tid + j * kThreads;
     bits[j] = r.mask && i < full ? mask_bits<N>(r.mask, first + i * N) : kAll;
   }
-  if (counted) count_history(r, first, n, counts);
   float v[PER][N];
   bool write[PER];
 #pragma unroll
@@ -40,14 +39,21 @@ __global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, Rul
     write[j] = i < full;
 #pragma unroll
     for (int e = 0; e < N; ++e) v[j][e] = -INFINITY;
-    if (write[j] && in_place && bits[j] == kAll) {
-      write[j] = false;
-      if (counted)
-#pragma unroll
-        for (int e = 0; e < N; ++e) write[j] |= counts[i * N + e] > 0;
-    }
-    if (write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
+    if (!in_place && write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
   }
+  if (counted) count_history(r, first, n, counts);
+  if (in_place)
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = tid + j * kThreads;
+      if (write[j] && bits[j] == kAll) {
+        write[j] = false;
+        if (counted)
+#pragma unroll
+          for (int e = 0; e < N; ++e) write[j] |= counts[i * N + e] > 0;
+      }
+      if (write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
+    }
   if (counted)
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
