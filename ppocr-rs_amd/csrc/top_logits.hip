@@ -11,6 +11,11 @@ __device__ __forceinline__ uint32_t value_key(float x) {
   const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
   return x != x ? 0xFFFFFFFEu : k;  // below the key of all ones, which no class has
 }
+// Of a number (no NaN), a few operations fewer.
+__device__ __forceinline__ uint32_t number_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
 __device__ __forceinline__ uint64_t order_key(float x, int c, int last) {
   return (uint64_t)value_key(x) << 32 | (uint32_t)(last ? c : ~c);
 }
@@ -224,10 +229,17 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
   ws = wave_sum(sum);
 }
 
+// Whether bf16 rows stay as stored: where widened ones would take the registers
+// of another wave.
+template <typename T, int PER, RuleParts RULES>
+constexpr bool top_raw() {
+  return RULES == kNoRules && PER * Pack<T>::N > 40;
+}
+
 // Waves a SIMD that the registers of a part leave room for.
 template <typename T, int NT, int PER, RuleParts RULES>
 constexpr int top_waves() {
-  constexpr int regs = RULES != kNoRules ? PER * Pack<T>::N : PER * 4;
+  constexpr int regs = top_raw<T, PER, RULES>() ? PER * 4 : PER * Pack<T>::N;
   if (NT == 1024 || (RULES == kNoRules && regs > 40)) return 4;
   if (RULES != kNoRules) return regs <= 40 ? 5 : 3;
   return regs <= 32 ? 7 : 4;
@@ -248,7 +260,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   if (tid == 0) sh.nan = 0;
 
   // Best logit of this thread and the first place that holds it.
-  RowPart<T, NT, PER, RULES == kNoRules> d;
+  RowPart<T, NT, PER, top_raw<T, PER, RULES>()> d;
   float high[PER];  // each pack's maximum
   float best = -INFINITY;
   int place = 0;
@@ -286,6 +298,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   const uint64_t bound = top_bound(sh, p.k);
   const float floor_value = key_value(bound);
   const uint32_t floor_place = (uint32_t)bound;
+  uint64_t* list = sh.list[wave];
   float wm = -INFINITY;
   double ws = 0.0;
   int n_wave = 0;
@@ -301,30 +314,39 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     const auto take = [&](float v, int at, int cls) {
       uint64_t lanes = lanes_where(v >= floor_value);
       if (!lanes) return false;
-      lanes &= lanes_where(v > floor_value) | lanes_where((uint32_t)~at >= floor_place);
+      if (floor_place) lanes &= lanes_where(v > floor_value) | lanes_where((uint32_t)~at >= floor_place);
       const bool mine = lanes >> lane & 1;
-      const int slot = n_wave + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
-      if (mine && slot < kList) sh.list[wave][slot] = order_key(v, cls, p.last_ties);
+      const int slot = __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, n_wave));
+      if (mine) list[min(slot, kList - 1)] = (uint64_t)number_key(v) << 32 | (uint32_t)(p.last_ties ? cls : ~cls);
       n_wave += __popcll(lanes);
       return mine;
     };
+    bool hits = false;
+    float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (!lanes_where(high[j] >= floor_value)) continue;
+      if (!lanes_where(high[j] >= floor_value)) {
+        m = fmaxf(m, high[j]);
+        continue;
+      }
+      hits = true;
       const int i = (seg * PER + j) * NT + tid;
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (take(d.pack[j].get(e), shape.pack_place(i), shape.pack_class(i) + e)) d.pack[j].clear(e);
-      high[j] = pack_max(d.pack[j]);
     }
     if (seg == 0 && take(d.tail, shape.tail_place(), shape.tail_class())) d.tail = -INFINITY;
-    float m = d.tail;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) m = fmaxf(m, high[j]);
-    m = wave_max(m);
-    // The maximum limited to finite numbers: +inf then counts as an infinite
-    // term and -inf as none.
-    const double sum = part_sum(d, fminf(fmaxf(m, -FLT_MAX), FLT_MAX), c);
+    // Terms relative to a limit of the wave's maximum: classes left in a pack
+    // that gave some to the list are at most the bound.  Far below it their sum
+    // would vanish, then the maximum itself is looked for.
+    m = fmaxf(wave_max(fmaxf(m, d.tail)), hits ? floor_value : -INFINITY);
+    double sum = part_sum(d, fminf(fmaxf(m, -FLT_MAX), FLT_MAX), c);
+    if (hits && sum < 0x1p-60) {
+      m = part_max(d);
+      // Limited to finite numbers: +inf then counts as an infinite term and -inf
+      // as none.
+      sum = part_sum(d, fminf(fmaxf(m, -FLT_MAX), FLT_MAX), c);
+    }
     if (sum != sum) sh.nan = 1;
     join_sums(wm, ws, fminf(m, FLT_MAX), sum, c);
   }
