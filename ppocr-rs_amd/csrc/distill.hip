@@ -28,9 +28,12 @@ __device__ __forceinline__ TeacherEntry teacher_entry(const DistillParams& p, in
 //   loss = tau^2 (sum_j q_j (log q_j - log p_j) + q0 (log q0 - log p0)),
 //   d loss / d s_c = tau (p_c - q_c) for an entry, tau e_c (1 / Z - q0 / Z0) else.
 // So the rest's gradient is e times one factor of the row, and the row is read
-// once: it stays in registers with the entries taken out (by marks in LDS).  Wave 0 does the entries, in 64 bits, the
-// teacher's shares while the row is on its way, and writes their gradients over
-// the row's.  The whole is formed from the rest and the entries, so that the
+// once: it stays in registers with the entries taken out (by marks in LDS).
+// Wave 0 does the entries, in 64 bits (the loss is a difference of logs that
+// nearly cancel), the teacher's shares while the row is on its way, and writes
+// their gradients over the row's; scalars of the row take lanes of the same
+// exponentials and logarithms, of which a batch of short rows would else do
+// little more.  The whole is formed from the rest and the entries, so that the
 // shares add up to one and an error of the rest's sum cancels to first order in
 // the loss.  Rows longer than the registers go through them in parts, twice when
 // the gradient is asked for.
@@ -40,8 +43,10 @@ struct DistillShared {
   double sum[16];
   float max[16];
   float factor, top;  // of the rest's gradient: exp((s - top) / tau) times factor
-  double q[64], logq[64];  // the teacher's shares, which wave 0 keeps here rather than in registers
-  double q0, logq0;
+  // The teacher's shares q, which wave 0 keeps here rather than in registers:
+  // log q = level - log(whole).
+  double q[64], level[64];
+  double q0, level0, whole;
 };
 
 // Waves a SIMD that the registers of a part leave room for.
@@ -50,25 +55,35 @@ constexpr int distill_waves() {
   return PER * 4 <= 16 ? 8 : 5;
 }
 
-// The teacher's shares of a row and their logs, by wave 0, in 64 bits: the loss
-// is a difference of logs that nearly cancel.  An entry that does not count
-// loses its index.
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The teacher's shares of a row, by wave 0.  An entry that does not count loses
+// its index.
 __device__ __forceinline__ void teacher_shares(const DistillParams& p, int64_t row, TeacherEntry& entry, double inv,
                                                bool maybe_again, DistillShared& sh) {
   const int lane = threadIdx.x & 63;
   // A class named twice counts once, with its first entry.
   bool again = false;
-  for (int j = 0; maybe_again && j + 1 < p.k; ++j) again |= __builtin_amdgcn_readlane(entry.index, j) == entry.index && j < lane;
+  for (int j = 0; maybe_again && j + 1 < p.k; ++j)
+    again |= __builtin_amdgcn_readlane(entry.index, j) == entry.index && j < lane;
   if (again) entry.index = -1;
   const bool valid = entry.index >= 0;
   const double rest = p.rest ? (double)p.rest[row] : -INFINITY;
   const double m = fmax((double)wave_max(valid ? entry.value : -INFINITY) * inv, rest);
-  const double d = (double)entry.value * inv - m;
-  const double x = valid ? exp(d) : 0.0, x0 = exp(rest - m);
-  const double sum = wave_sum(x) + x0, logsum = log(sum);
-  sh.q[lane] = x / sum;
-  sh.logq[lane] = d - logsum;
-  if (lane == 0) sh.q0 = x0 / sum, sh.logq0 = rest - m - logsum;
+  const double d = (double)entry.value * inv - m, d0 = rest - m;
+  // The rest takes the last lane where it holds no entry.
+  const bool spare = p.k < 64;
+  const double x = exp(spare && lane == 63 ? d0 : d);
+  const double x0 = spare ? lane_value(x, 63) : exp(d0);
+  const double whole = wave_sum(valid ? x : 0.0) + x0, share = 1.0 / whole;
+  sh.q[lane] = valid ? x * share : 0.0;
+  sh.level[lane] = d;
+  if (lane == 0) sh.q0 = x0 * share, sh.level0 = d0, sh.whole = whole;
 }
 
 // Marks of the entries' classes below the row's last classes % N: a bit a class,
@@ -110,10 +125,7 @@ struct Marks {
       for (int j = 0; j < PER; ++j) {
         const int i = (seg * PER + j) * NT + (int)threadIdx.x;
         const unsigned bits = i < shape.full ? mask_bits<N>(at, i * N) : 0;
-        if (bits)
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (bits >> e & 1) d.pack[j].clear(e);
+        if (bits) d.pack[j].drop(bits);
       }
     } else {
 #pragma unroll
@@ -121,10 +133,7 @@ struct Marks {
         const uint32_t word = at[threadIdx.x * kWords + w];
         if (word)
 #pragma unroll
-          for (int q = 0; q < 4 && w * 4 + q < PER; ++q)
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (word >> (q * 8 + e) & 1) d.pack[w * 4 + q].clear(e);
+          for (int q = 0; q < 4 && w * 4 + q < PER; ++q) d.pack[w * 4 + q].drop(word >> (q * 8));
       }
     }
   }
@@ -182,7 +191,10 @@ __global__ __launch_bounds__(NT, distill_waves<PER>()) void distill_kernel(Logit
       float pm = part_max(d);
       const double ps = part_sum(d, fmaxf(pm, -FLT_MAX), c);
       if (ps != ps) pm = fmaxf(pm, -FLT_MAX);  // a NaN is no maximum but must not be lost
-      join_sums(m, sum, pm, ps, c);
+      if (PARTS)
+        join_sums(m, sum, pm, ps, c);
+      else
+        m = pm, sum = ps;
     }
     if (lane == 0) sh.max[wave] = m, sh.sum[wave] = sum;
     __syncthreads();
@@ -194,26 +206,29 @@ __global__ __launch_bounds__(NT, distill_waves<PER>()) void distill_kernel(Logit
     const bool valid = entry.index >= 0;
     const double q = sh.q[lane], q0 = sh.q0;
     double top, z, mr, zr;
+    float om = -INFINITY;
     if constexpr (MODE == kGradient) {
       const float* st = p.state + row * 4;
       top = st[0], z = st[1], mr = st[2], zr = st[3];
     } else {
-      const float om = lane < W ? sh.max[lane] : -INFINITY;
-      const float rm = wave_max(om);
-      zr = wave_sum(om > -INFINITY ? sh.sum[lane] * exp(((double)om - rm) * inv) : 0.0);
-      mr = rm;
-      top = fmaxf(rm, wave_max(valid ? own : -INFINITY));
+      if (lane < W) om = sh.max[lane];
+      mr = wave_max(om);
+      top = fmaxf((float)mr, wave_max(valid ? own : -INFINITY));
     }
     const double low = fmax(top, -(double)FLT_MAX);
-    const double a = ((double)own - low) * inv;
+    const double a = ((double)own - low) * inv, a0 = (mr - low) * inv;
     const double e = valid ? exp(a) : 0.0;
-    const double e0 = mr == -INFINITY ? 0.0 : exp((mr - low) * inv);  // of the rest's maximum
+    // Of the rest's maximum in the last lane, of the waves' in theirs.
+    const double joint = exp(lane < W ? ((double)om - mr) * inv : a0);
+    const double e0 = mr == -INFINITY ? 0.0 : lane_value(joint, 63);
     if constexpr (MODE != kGradient) {
+      zr = wave_sum(om > -INFINITY ? sh.sum[lane] * joint : 0.0);
       z = wave_sum(e) + zr * e0;
-      const double logz = log(z);
-      double term = valid && q > 0.0 ? q * (sh.logq[lane] - (a - logz)) : 0.0;
+      const double logs = log(lane == 0 ? z : lane == 1 ? zr : sh.whole);
+      const double logz = lane_value(logs, 0), logzr = lane_value(logs, 1), logwhole = lane_value(logs, 2);
+      double term = valid && q > 0.0 ? q * (sh.level[lane] - logwhole - (a - logz)) : 0.0;
       if (lane == 0 && q0 > 0.0)
-        term += q0 * (sh.logq0 - (zr > 0.0 || zr != zr ? (mr - low) * inv + log(zr) - logz : -INFINITY));
+        term += q0 * (sh.level0 - logwhole - (zr > 0.0 || zr != zr ? a0 + logzr - logz : -INFINITY));
       const double loss = wave_sum(term) * (double)p.temperature * (double)p.temperature;
       if (lane == 0) {
         p.loss[row] = top == -INFINITY && !(z != z) ? INFINITY : (float)loss;
@@ -231,8 +246,9 @@ __global__ __launch_bounds__(NT, distill_waves<PER>()) void distill_kernel(Logit
       const bool dead = top == -INFINITY && !(z != z);
       // Of exponentials relative to the rest's maximum: its classes may be far
       // below the entries and still share q0 among them.
-      const double factor = dead || zr == 0.0 ? 0.0 : scale * (e0 / z - q0 / zr);
-      entry_grad = dead ? 0.0f : (float)(scale * (e / z - q));
+      const double share = 1.0 / z;
+      const double factor = dead || zr == 0.0 ? 0.0 : scale * (e0 * share - q0 / zr);
+      entry_grad = dead ? 0.0f : (float)(scale * (e * share - q));
       if (lane == 0) sh.factor = (float)factor, sh.top = (float)fmax(mr, -(double)FLT_MAX);
     }
   }

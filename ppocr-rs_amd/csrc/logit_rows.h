@@ -118,12 +118,12 @@ struct PackRegs {
   __device__ __forceinline__ void load(const T* p) { Pack<T>::load(p, v); }
   __device__ __forceinline__ float get(int e) const { return v[e]; }
   __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
-  // Elements whose bit is 0 become -inf: a bit stretched over the word selects.
-  __device__ __forceinline__ void keep(unsigned bits) {
+  // Elements whose bit is set become -inf: a bit stretched over the word selects.
+  __device__ __forceinline__ void drop(unsigned bits) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const uint32_t m = (uint32_t)((int)(bits << (31 - e)) >> 31);
-      v[e] = __uint_as_float((__float_as_uint(v[e]) & m) | (0xFF800000u & ~m));
+      v[e] = __uint_as_float((__float_as_uint(v[e]) & ~m) | (0xFF800000u & m));
     }
   }
   __device__ __forceinline__ void clear(int e) { v[e] = -INFINITY; }
@@ -144,6 +144,14 @@ struct PackRegs<bf16, true> {
   }
   __device__ __forceinline__ void clear(int e) {
     v[e >> 1] = e & 1 ? (v[e >> 1] & 0xFFFFu) | 0xFF800000u : (v[e >> 1] & 0xFFFF0000u) | 0xFF80u;
+  }
+  __device__ __forceinline__ void drop(unsigned bits) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = (uint32_t)((int)(bits << (31 - 2 * i)) >> 31), hi = (uint32_t)((int)(bits << (30 - 2 * i)) >> 31);
+      const uint32_t m = (lo & 0xFFFFu) | hi << 16;
+      v[i] = (v[i] & ~m) | (0xFF80FF80u & m);
+    }
   }
   __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0xFF80FF80u; }
   // Widened values are not kept past here: twice the registers would be live.
