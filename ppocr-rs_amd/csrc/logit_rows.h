@@ -69,36 +69,43 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // ------------------------------------------------------------------ packs
-// 16 bytes of a row, at any alignment of the element.
+// 16 bytes of a row as stored, read at any alignment of the element.  All packs
+// of a thread are read before the first is widened: a use right after its load
+// would make each load wait for the one before.
+struct PackBits {
+  uint32_t v[4];
+};
+
 template <typename T>
 struct Pack;
 template <>
 struct Pack<float> {
   static constexpr int N = 4;
-  typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const Raw r = *reinterpret_cast<const Raw*>(p);
-    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(4)));
+  static __device__ __forceinline__ PackBits none() {
+    return PackBits{{0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u}};
+  }
+  static __device__ __forceinline__ void widen(const PackBits& b, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(b.v[i]);
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-    *reinterpret_cast<Raw*>(p) = Raw{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<Raw*>(p) =
+        Raw{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
   }
 };
 template <>
 struct Pack<bf16> {
   static constexpr int N = 8;
   typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
-  static __device__ __forceinline__ void load(const bf16* p, uint32_t (&v)[4]) {
-    const Raw r = *reinterpret_cast<const Raw*>(p);
-    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  static __device__ __forceinline__ PackBits none() {
+    return PackBits{{0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u}};
   }
-  static __device__ __forceinline__ void load(const bf16* p, float (&v)[8]) {
-    uint32_t r[4];
-    load(p, r);
+  static __device__ __forceinline__ void widen(const PackBits& b, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(r[i] << 16);
-      v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+      v[2 * i] = __uint_as_float(b.v[i] << 16);
+      v[2 * i + 1] = __uint_as_float(b.v[i] & 0xFFFF0000u);
     }
   }
   static __device__ __forceinline__ void store(bf16* p, const float (&v)[8]) {
@@ -108,6 +115,11 @@ struct Pack<bf16> {
     *reinterpret_cast<Raw*>(p) = r;
   }
 };
+template <typename T>
+__device__ __forceinline__ PackBits load_pack(const T* p) {
+  const typename Pack<T>::Raw r = *reinterpret_cast<const typename Pack<T>::Raw*>(p);
+  return PackBits{{r.x, r.y, r.z, r.w}};
+}
 
 // One pack in registers: fp32, or bf16 as stored (half the registers; each
 // use widens it with one operation), which cannot hold what rules make of it.
@@ -115,10 +127,18 @@ template <typename T, bool RAW>
 struct PackRegs {
   static constexpr int N = Pack<T>::N;
   float v[N];
-  __device__ __forceinline__ void load(const T* p) { Pack<T>::load(p, v); }
+  __device__ __forceinline__ void take(const PackBits& b) { Pack<T>::widen(b, v); }
   __device__ __forceinline__ float get(int e) const { return v[e]; }
   __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
-  // Elements whose bit is set become -inf: a bit stretched over the word selects.
+  // Elements whose bit is 0, or is set, become -inf: a bit stretched over the
+  // word selects.
+  __device__ __forceinline__ void keep(unsigned bits) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const uint32_t m = (uint32_t)((int)(bits << (31 - e)) >> 31);
+      v[e] = __uint_as_float((__float_as_uint(v[e]) & m) | (0xFF800000u & ~m));
+    }
+  }
   __device__ __forceinline__ void drop(unsigned bits) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -127,10 +147,6 @@ struct PackRegs {
     }
   }
   __device__ __forceinline__ void clear(int e) { v[e] = -INFINITY; }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = -INFINITY;
-  }
   template <int AT = 0>
   __device__ __forceinline__ void forget() {}
 };
@@ -138,7 +154,10 @@ template <>
 struct PackRegs<bf16, true> {
   static constexpr int N = 8;
   uint32_t v[4];
-  __device__ __forceinline__ void load(const bf16* p) { Pack<bf16>::load(p, v); }
+  __device__ __forceinline__ void take(const PackBits& b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = b.v[i];
+  }
   __device__ __forceinline__ float get(int e) const {
     return __uint_as_float(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
   }
@@ -153,7 +172,6 @@ struct PackRegs<bf16, true> {
       v[i] = (v[i] & ~m) | (0xFF80FF80u & m);
     }
   }
-  __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0xFF80FF80u; }
   // Widened values are not kept past here: twice the registers would be live.
   // (AT tells two branches apart, whose beginnings would be joined.)
   template <int AT = 0>
@@ -205,15 +223,16 @@ struct RowShape {
 template <typename P, typename T, int N>
 __device__ __forceinline__ void load_part(P& d, const T* x, const RowShape<N>& s, int seg,
                                           const unsigned* bits = nullptr) {
+  PackBits b[P::kPer];
 #pragma unroll
   for (int j = 0; j < P::kPer; ++j) {
     const int i = (seg * P::kPer + j) * P::kThreads + (int)threadIdx.x;
-    if (bits ? bits[j] != 0 : i < s.full)
-      d.pack[j].load(x + s.pack_class(i));
-    else
-      d.pack[j].clear();
+    b[j] = Pack<T>::none();
+    if (bits ? bits[j] != 0 : i < s.full) b[j] = load_pack(x + s.pack_class(i));
   }
   d.tail = seg == 0 && s.has_tail() ? ld1<T>(x + s.tail_class()) : -INFINITY;
+#pragma unroll
+  for (int j = 0; j < P::kPer; ++j) d.pack[j].take(b[j]);
 }
 
 // exp((x - m) / tau) for many x: 2^(x c - b) with c = log2(e) / tau and b = m c
@@ -336,7 +355,7 @@ __device__ __forceinline__ void load_bias(const float* p, float (&v)[N]) {
 #pragma unroll
   for (int q = 0; q < N; q += 4) {
     float b[4];
-    Pack<float>::load(p + q, b);
+    Pack<float>::widen(load_pack(p + q), b);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[q + e] = b[e];
   }

@@ -31,15 +31,14 @@ __global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, Rul
     const int i = tid + j * kThreads;
     bits[j] = r.mask && i < full ? mask_bits<N>(r.mask, first + i * N) : kAll;
   }
-  float v[PER][N];
+  PackBits raw[PER];
   bool write[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = tid + j * kThreads;
     write[j] = i < full;
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[j][e] = -INFINITY;
-    if (!in_place && write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
+    raw[j] = Pack<T>::none();
+    if (!in_place && write[j] && bits[j]) raw[j] = load_pack(x + i * N);
   }
   if (counted) count_history(r, first, n, counts);
   if (in_place)
@@ -52,8 +51,11 @@ __global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, Rul
 #pragma unroll
           for (int e = 0; e < N; ++e) write[j] |= counts[i * N + e] > 0;
       }
-      if (write[j] && bits[j]) Pack<T>::load(x + i * N, v[j]);
+      if (write[j] && bits[j]) raw[j] = load_pack(x + i * N);
     }
+  float v[PER][N];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) Pack<T>::widen(raw[j], v[j]);
   if (counted)
 #pragma unroll
     for (int j = 0; j < PER; ++j) {

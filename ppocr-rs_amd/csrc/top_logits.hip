@@ -106,7 +106,7 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
     }
     if (r.mask) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) d.pack[j].drop(~bits[j]);
+      for (int j = 0; j < PER; ++j) d.pack[j].keep(bits[j]);
       if (seg == 0 && s.has_tail() && !mask_bit(r.mask, s.tail_class())) d.tail = -INFINITY;
     }
   }
