@@ -156,7 +156,7 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
   uint32_t lo = max(kNone + 1, wave_min(min(min(key[0], key[1]), min(key[2], key[3]))));
   uint32_t hi = wave_max(max(max(key[0], key[1]), max(key[2], key[3]))) + 1;
   int n = kGroups;
-  const int enough = k + k / 2 + 8;
+  const int enough = k + k / 8 + 4;
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
     const int c = reach(mid);
