@@ -81,7 +81,10 @@ def test_ruled_recognizers(gpu, size, precision, parts):
         assert np.all(np.abs(g[..., 1] - got.max(-1)) <= REL * got.max(-1))
         t = top.forward(x).array()
         assert t.shape == p.shape[:2] + (20, 2)
-        assert np.array_equal(t[..., 0, :], g)
+        # Another k splits the sum between listed classes and the rest elsewhere:
+        # the same class, its probability within the sums' roundings.
+        assert np.array_equal(t[..., 0, 0], g[..., 0])
+        assert np.all(np.abs(t[..., 0, 1] - g[..., 1]) <= REL * g[..., 1])
         assert (np.diff(t[..., 1], axis=-1) <= 0).all()
         classes = t[..., 0].astype(np.int64)
         assert np.all(np.abs(np.take_along_axis(got, classes, -1) - t[..., 1]) <= REL * t[..., 1] + TINY)
