@@ -229,20 +229,13 @@ __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int cl
   ws = wave_sum(sum);
 }
 
-// Whether bf16 rows stay as stored: where widened ones would take the registers
-// of another wave.
-template <typename T, int PER, RuleParts RULES>
-constexpr bool top_raw() {
-  return RULES == kNoRules && PER * Pack<T>::N > 40;
-}
-
 // Waves a SIMD that the registers of a part leave room for.
 template <typename T, int NT, int PER, RuleParts RULES>
 constexpr int top_waves() {
-  constexpr int regs = top_raw<T, PER, RULES>() ? PER * 4 : PER * Pack<T>::N;
-  if (NT == 1024 || (RULES == kNoRules && regs > 40)) return 4;
-  if (RULES != kNoRules) return regs <= 40 ? 5 : 3;
-  return regs <= 32 ? 7 : 4;
+  constexpr int regs = PER * Pack<T>::N;
+  if (NT == 1024) return 4;
+  if (regs <= 32) return RULES == kNoRules ? 7 : 5;
+  return regs <= 40 ? 5 : RULES == kNoRules ? 4 : 3;
 }
 
 template <typename T, int NT, int PER, RuleParts RULES>
@@ -260,7 +253,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   if (tid == 0) sh.nan = 0;
 
   // Best logit of this thread and the first place that holds it.
-  RowPart<T, NT, PER, top_raw<T, PER, RULES>()> d;
+  RowPart<T, NT, PER, false> d;
   float high[PER];  // each pack's maximum
   float best = -INFINITY;
   int place = 0;
@@ -302,7 +295,6 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   float wm = -INFINITY;
   double ws = 0.0;
   int n_wave = 0;
-  d.forget();
   for (int seg = parts - 1; seg >= 0; --seg) {
     if (seg != parts - 1) {
       read_part<RULES>(d, x, r, shape, seg, counts);
