@@ -298,15 +298,17 @@ void launch_distill_one(const LogitRows& in, const DistillParams& p, hipStream_t
 // Threads of a row's workgroup and the elements that each holds.  512 threads
 // of 40 elements keep more waves on a CU than 256 of 80 (2560 x 18710 fp32, loss
 // and gradient: 80 us against 105), but for the loss alone of bf16 batches,
-// whose rows take half the registers (10240 x 18710: 92 us against 109).
+// whose rows take half the registers (10240 x 18710: 92 us against 109).  Now
+// 2560 x 18710 fp32: loss 31.5 us (6.1 TB/s), gradient 75 us (5.1), both 79 us
+// (4.9); 10240 x 18710 bf16: 81 us (4.8), 140 us (5.5), 157 us (4.9).
 template <typename T, DistillMode MODE>
 void launch_distill_typed(const LogitRows& in, const DistillParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N;
-  constexpr bool kSlim = MODE == kLoss && sizeof(T) == 2;
+  if constexpr (MODE == kLoss && sizeof(T) == 2)
+    if (in.rows >= 1024 && in.classes > 256 * 32 && in.classes <= 256 * 80)
+      return launch_distill_one<T, 256, 80 / N, false, MODE>(in, p, s);
   if (in.classes <= 256 * 8 || (in.rows >= 1024 && in.classes <= 256 * 32))
     launch_distill_one<T, 256, 32 / N, false, MODE>(in, p, s);
-  else if (kSlim && in.rows >= 1024 && in.classes <= 256 * 80)
-    launch_distill_one<bf16, 256, 80 / 8, false, kLoss>(in, p, s);
   else if (in.classes <= 512 * 40)
     launch_distill_one<T, 512, 40 / N, false, MODE>(in, p, s);
   else if (in.classes <= 1024 * 40)

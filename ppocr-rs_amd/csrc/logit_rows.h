@@ -161,9 +161,6 @@ struct PackRegs<bf16, true> {
   __device__ __forceinline__ float get(int e) const {
     return __uint_as_float(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
   }
-  __device__ __forceinline__ void clear(int e) {
-    v[e >> 1] = e & 1 ? (v[e >> 1] & 0xFFFFu) | 0xFF800000u : (v[e >> 1] & 0xFFFF0000u) | 0xFF80u;
-  }
   __device__ __forceinline__ void drop(unsigned bits) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -279,8 +276,8 @@ __device__ __forceinline__ float part_max(const P& d) {
   return wave_max(m);
 }
 
-// Sums of exp((x - max) * c) with their own maxima, joined: (m, s) becomes the
-// sum of both.  -inf is no maximum.
+// Sums of exp((x - m) * c) with a reference m each, joined: (m, s) becomes the
+// sum of both.  A reference of -inf has no terms.
 __device__ __forceinline__ void join_sums(float& m, double& s, float om, double os, float c) {
   const float nm = fmaxf(m, om);
   if (nm == -INFINITY) return;

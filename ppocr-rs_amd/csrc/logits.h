@@ -12,8 +12,8 @@
 
 namespace ppocr {
 
-// Largest number of classes of a row and largest k: the top kernel keeps the
-// elements of k threads, at most k * ceil(classes / threads) candidates, in LDS.
+// Largest number of classes of a row (the marks of a row take 32 KB of LDS) and
+// largest k (an entry a lane of a wave).
 constexpr int kMaxLogitClasses = 1 << 18;
 constexpr int kMaxTop = 64;
 

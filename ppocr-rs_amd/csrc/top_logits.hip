@@ -113,7 +113,11 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
 }
 
 // The k best classes of a row and the log-sum-exp of the others, one row a
-// workgroup, the row read once (parts of longer rows a second time).
+// workgroup, the row read once (parts of longer rows a second time).  fp32 rows
+// are bound by HBM (10240 x 18710, top 8: 133 us, 5.8 TB/s), bf16 ones and long
+// lists by vector work, some 1000 to 1700 operations a wave, a third of them
+// exponentials (the same in bf16, top 8: 94 us, top 64: 128 us, where HBM would
+// take 70).
 //
 // Every group of NT / 256 threads has its best (logit, first place that holds
 // it).  The k-th best of the 256 groups bounds the k-th best class from below,
@@ -329,11 +333,12 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     }
     if (seg == 0 && take(d.tail, shape.tail_place(), shape.tail_class())) d.tail = -INFINITY;
     // Terms relative to a limit of the wave's maximum: classes left in a pack
-    // that gave some to the list are at most the bound.  Far below it their sum
-    // would vanish, then the maximum itself is looked for.
+    // that gave some to the list are at most the bound.  Where they are so far
+    // below it that the terms' arguments would lose digits, the maximum itself is
+    // looked for.
     m = fmaxf(wave_max(fmaxf(m, d.tail)), hits ? floor_value : -INFINITY);
     double sum = part_sum(d, fminf(fmaxf(m, -FLT_MAX), FLT_MAX), c);
-    if (hits && sum < 0x1p-60) {
+    if (hits && sum < 0.25) {
       m = part_max(d);
       // Limited to finite numbers: +inf then counts as an infinite term and -inf
       // as none.
@@ -412,9 +417,9 @@ void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
 
 // Threads of a row's workgroup and the elements that each holds.  A few hundred
 // rows fill the chip better with 512 threads (378 x 18710 fp32 under masks, top
-// 3: 14.5 us against 20.4 with 1024 and 20.8 with 256), batches with 256, whose
-// waves share the work of bound and ranking (10240 x 18710 fp32, top 64: 149 us
-// against 223 with 512).
+// 3: 14.5 us against 20.4 with 1024), batches with 256, where fewer waves repeat
+// the search for the bound (10240 x 18710 fp32, top 64: 149 us against 223 with
+// 512).
 template <typename T, RuleParts RULES>
 void launch_top_rules(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N, kLong = RULES != kNoRules ? 64 : 80;
