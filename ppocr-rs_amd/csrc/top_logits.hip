@@ -119,47 +119,62 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
 // exponentials (the same in bf16, top 8: 94 us, top 64: 128 us, where HBM would
 // take 70).
 //
-// Every group of NT / 256 threads has its best (logit, first place that holds
-// it).  The k-th best of the 256 groups bounds the k-th best class from below,
-// and only about k groups hold classes above the bound: those leave the
-// registers for a list of the wave in LDS, and each finds its rank by counting
-// the better ones in all lists.  What is left in the registers and the end of
-// the ranking is the rest.  The bound is found by bisection over the groups'
-// order keys, every wave for itself.  Lists that overflow (rows whose best
-// classes crowd in few threads) or a NaN (which shows in the sums) send the row
-// to k searches for the next best class.
-constexpr int kGroups = 256, kList = 256, kSorted = 512;
+// The classes form groups, each with its best (logit, first place that holds
+// it).  The k-th best group bounds the k-th best class from below, and only
+// about k groups hold classes above the bound: those leave the registers for a
+// list of the wave in LDS, and each finds its rank by counting the better ones
+// in all lists.  What is left in the registers and the end of the ranking is the
+// rest.  The bound is found by bisection over the groups' order keys, every wave
+// for itself.  Lists that overflow (rows whose best classes crowd in few
+// threads) or a NaN (which shows in the sums) send the row to k searches for the
+// next best class.
+//
+// Groups: of several waves 256, each of NT / 256 threads' classes, or the
+// threads themselves where a mask leaves candidates to k groups or fewer (all of
+// these would be listed); of a single wave its packs, or its classes where it
+// holds eight a lane.
+constexpr int kSorted = 512;
 
-template <int W>
+template <int NT>
 struct TopShared {
-  alignas(16) uint64_t list[W][kList];
-  uint64_t sorted[kSorted];
-  uint32_t group_key[kGroups], group_place[kGroups];
+  static constexpr int kThreadKeys = NT > 256 ? NT : 0;
+  union {
+    struct {
+      uint32_t key[256 + kThreadKeys], place[256 + kThreadKeys];
+    } group;
+    uint64_t sorted[kSorted];  // written when the groups are done with
+  };
   uint64_t red[16];
   double wave_sum[16];
   float wave_max[16];
-  int count[W];  // of the waves' lists
+  int count[16];  // of the waves' lists
   int nan;
 };
+// Room of a wave's list: k groups that are a wave's packs, all of whose classes
+// pass, or half of it where sixteen waves' lists of as many fp32 classes fit.
+template <int NT, int N>
+constexpr int top_list() {
+  return NT == 1024 && N == 4 ? 256 : 512;
+}
 
-// Bound of the list: the composite (value key, ~place) that at least k groups
-// reach, and few more.
-template <int W>
-__device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
-  const int lane = threadIdx.x & 63;
-  uint32_t key[4], place[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) key[i] = sh.group_key[i * 64 + lane], place[i] = sh.group_place[i * 64 + lane];
+// Bound of the list: the composite (value key, ~place) that at least k of the
+// wave's groups, K a lane, reach, and few more.  0: only k groups or fewer hold
+// a candidate.
+template <int K>
+__device__ __forceinline__ uint64_t top_bound(const uint32_t (&key)[K], const uint32_t (&place)[K], int k) {
   const auto reach = [&](uint32_t t) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += __popcll(lanes_where(key[i] >= t));
+    for (int i = 0; i < K; ++i) n += __popcll(lanes_where(key[i] >= t));
     return n;
   };
-  if (reach(kNone + 1) <= k) return (uint64_t)(kNone + 1) << 32;
-  uint32_t lo = max(kNone + 1, wave_min(min(min(key[0], key[1]), min(key[2], key[3]))));
-  uint32_t hi = wave_max(max(max(key[0], key[1]), max(key[2], key[3]))) + 1;
-  int n = kGroups;
+  int n = reach(kNone + 1);
+  if (n <= k) return 0;
+  uint32_t least = key[0], most = key[0];
+#pragma unroll
+  for (int i = 1; i < K; ++i) least = min(least, key[i]), most = max(most, key[i]);
+  uint32_t lo = max(kNone + 1, wave_min(least));
+  uint32_t hi = wave_max(most) + 1;
   const int enough = k + k / 8 + 4;
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
@@ -180,7 +195,7 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
     const uint32_t mid = plo + (phi - plo) / 2;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c += __popcll(lanes_where(key[i] == lo && place[i] >= mid));
+    for (int i = 0; i < K; ++i) c += __popcll(lanes_where(key[i] == lo && place[i] >= mid));
     if (c >= need)
       plo = mid;
     else
@@ -191,9 +206,9 @@ __device__ __forceinline__ uint64_t top_bound(const TopShared<W>& sh, int k) {
 
 // The slow way for any row: k searches for the best class below the last one,
 // then the sums of the others, the row read each time.
-template <typename T, RuleParts RULES, int W>
+template <typename T, RuleParts RULES, int NT>
 __device__ __forceinline__ void search_row(const T* x, const RowRules& r, int classes, const TopParams& p, float c,
-                                           int* counts, TopShared<W>& sh, float& wm, double& ws) {
+                                           int* counts, TopShared<NT>& sh, float& wm, double& ws) {
   const auto each = [&](auto&& f) {
     for (int first = 0; first < classes; first += kWindow) {
       const int n = min(kWindow, classes - first);
@@ -244,9 +259,10 @@ constexpr int top_waves() {
 
 template <typename T, int NT, int PER, RuleParts RULES>
 __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logits_kernel(LogitRows in, TopParams p, int parts) {
-  constexpr int N = Pack<T>::N, W = NT / 64;
-  __shared__ TopShared<W> sh;
-  extern __shared__ int counts[];
+  constexpr int N = Pack<T>::N, W = NT / 64, kList = top_list<NT, N>();
+  __shared__ TopShared<NT> sh;
+  extern __shared__ __align__(16) uint64_t lists[];  // [W][kList], then the history's counters
+  int* counts = reinterpret_cast<int*>(lists + W * kList);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(in.x) + row * in.stride;
@@ -271,31 +287,66 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     read_part<RULES>(d, x, r, shape, seg, counts);
     if (seg == 0) {
       tail = d.tail;
-      if (shape.last) look(tail, shape.tail_place());
+      if (W > 1 && shape.last) look(tail, shape.tail_place());
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       high[j] = pack_max(d.pack[j]);
-      look(high[j], shape.pack_place((seg * PER + j) * NT + tid));
+      if (W > 1) look(high[j], shape.pack_place((seg * PER + j) * NT + tid));
     }
   }
-  if (!shape.last) look(tail, shape.tail_place());
-  uint64_t mine = (uint64_t)value_key(best) << 32 | (uint32_t)~place;
-  if constexpr (NT > kGroups) {
+  uint64_t bound;
+  if constexpr (W > 1) {
+    if (!shape.last) look(tail, shape.tail_place());
+    uint64_t mine = (uint64_t)value_key(best) << 32 | (uint32_t)~place;
+    constexpr int S = NT / 256;
+    if constexpr (S > 1) {
+      sh.group.key[256 + tid] = (uint32_t)(mine >> 32);
+      sh.group.place[256 + tid] = (uint32_t)mine;
 #pragma unroll
-    for (int o = 1; o < NT / kGroups; o <<= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
+      for (int o = 1; o < S; o <<= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
+    }
+    if (tid % S == 0) {
+      sh.group.key[tid / S] = (uint32_t)(mine >> 32);
+      sh.group.place[tid / S] = (uint32_t)mine;
+    }
+    __syncthreads();
+    uint32_t keys[4], places[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keys[i] = sh.group.key[i * 64 + lane], places[i] = sh.group.place[i * 64 + lane];
+    bound = top_bound(keys, places, p.k);
+    if constexpr (S > 1) {
+      if (!bound) {
+        uint32_t all[W], at[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) all[i] = sh.group.key[256 + i * 64 + lane], at[i] = sh.group.place[256 + i * 64 + lane];
+        bound = top_bound(all, at, p.k);
+      }
+    }
+  } else {
+    // A single wave, whose row is one part: its packs, or its classes.
+    constexpr bool kClassGroups = PER * N <= 8;
+    constexpr int K = (kClassGroups ? PER * N : PER) + 1;
+    uint32_t keys[K], places[K];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t at = (uint32_t)~shape.pack_place(j * NT + tid);
+      if constexpr (kClassGroups) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) keys[j * N + e] = value_key(d.pack[j].get(e)), places[j * N + e] = at;
+      } else {
+        keys[j] = value_key(high[j]), places[j] = at;
+      }
+    }
+    keys[K - 1] = value_key(tail), places[K - 1] = (uint32_t)~shape.tail_place();
+    bound = top_bound(keys, places, p.k);
   }
-  if (tid % (NT / kGroups) == 0) {
-    sh.group_key[tid / (NT / kGroups)] = (uint32_t)(mine >> 32);
-    sh.group_place[tid / (NT / kGroups)] = (uint32_t)mine;
-  }
-  __syncthreads();
+  if (!bound) bound = (uint64_t)(kNone + 1) << 32;  // every candidate
 
   // Classes above the bound go to the wave's list; the others' sums.
-  const uint64_t bound = top_bound(sh, p.k);
   const float floor_value = key_value(bound);
   const uint32_t floor_place = (uint32_t)bound;
-  uint64_t* list = sh.list[wave];
+  uint64_t* list = lists + wave * kList;
   float wm = -INFINITY;
   double ws = 0.0;
   int n_wave = 0;
@@ -349,7 +400,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   }
   if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws, sh.count[wave] = n_wave;
   // Zeros behind the list, to the next eight.
-  if (lane < 8 && n_wave + lane < kList) sh.list[wave][n_wave + lane] = 0;
+  if (lane < 8 && n_wave + lane < kList) list[n_wave + lane] = 0;
   __syncthreads();
 
   int n = 0, most = 0;
@@ -359,16 +410,16 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     for (int i = tid; i < n; i += NT) {
       int from = 0, at = i;
       while (at >= sh.count[from]) at -= sh.count[from++];
-      const uint64_t key = sh.list[from][at];
+      const uint64_t key = lists[from * kList + at];
       int rank = 0;
       for (int w = 0; w < W; ++w)
         for (int o = 0; o < sh.count[w]; o += 8)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) rank += sh.list[w][o + q] > key;
+          for (int q = 0; q < 8; ++q) rank += lists[w * kList + o + q] > key;
       sh.sorted[rank] = key;
     }
   } else {
-    search_row<T, RULES, W>(x, r, in.classes, p, c, counts, sh, wm, ws);
+    search_row<T, RULES, NT>(x, r, in.classes, p, c, counts, sh, wm, ws);
     n = p.k;
     if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws;
   }
@@ -410,25 +461,39 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
 template <typename T, int NT, int PER, RuleParts RULES>
 void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int kClasses = NT * PER * Pack<T>::N;
-  const size_t lds = RULES == kHistory ? (kWindow + 8) * sizeof(int) : 0;
+  const size_t lds = (size_t)NT / 64 * top_list<NT, Pack<T>::N>() * sizeof(uint64_t) +
+                     (RULES == kHistory ? (kWindow + 8) * sizeof(int) : 0);
   hipLaunchKernelGGL((top_logits_kernel<T, NT, PER, RULES>), dim3((unsigned)in.rows), dim3(NT), lds, s, in, p,
                      (in.classes + kClasses - 1) / kClasses);
 }
 
-// Threads of a row's workgroup and the elements that each holds.  A few hundred
-// rows fill the chip better with 512 threads (378 x 18710 fp32 under masks, top
-// 3: 14.5 us against 20.4 with 1024), batches with 256, where fewer waves repeat
-// the search for the bound (10240 x 18710 fp32, top 64: 149 us against 223 with
-// 512).
+// Threads of a row's workgroup and the elements that each holds.  Short rows
+// take a wave, which waits for no other (20000 x 300 fp32, top 64: 49 us against
+// 111 with 256 threads), with 32 elements a thread where there are rows enough
+// to hide its latency (10000 x 1900, top 8: 31 us against 48; 300 x 1000 10
+// against 8.7).  A few hundred rows fill the chip better with 512 threads (378 x
+// 18710 fp32 under masks, top 3: 14.5 us against 20.4 with 1024), batches with
+// 256, where fewer waves repeat the search for the bound (10240 x 18710 fp32,
+// top 64: 149 us against 223 with 512).  Longer rows are read twice in parts
+// rather than held by 1024 threads, whose one workgroup leaves its CU idle at
+// each wait (700 x 70000 fp32: 52 us against 57, 1500 x 30001 in one part 42
+// against 80), but where rules would be applied twice too (256 x 131072 under
+// masks 37 against 54) or few rows leave CUs idle.
 template <typename T, RuleParts RULES>
 void launch_top_rules(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int N = Pack<T>::N, kLong = RULES != kNoRules ? 64 : 80;
-  if (in.rows < 1024 && in.classes > 256 * 8 && in.classes <= 512 * 40)
+  if (in.classes <= 64 * 8)
+    launch_top<T, 64, 8 / N, RULES>(in, p, s);
+  else if (in.rows >= 1024 && in.classes <= 64 * 32)
+    launch_top<T, 64, 32 / N, RULES>(in, p, s);
+  else if (in.rows < 1024 && in.classes > 64 * 32 && in.classes <= 512 * 40)
     launch_top<T, 512, 40 / N, RULES>(in, p, s);
   else if (in.classes <= 256 * 32)
     launch_top<T, 256, 32 / N, RULES>(in, p, s);
   else if (in.classes <= 256 * 80)
     launch_top<T, 256, 80 / N, RULES>(in, p, s);
+  else if (in.classes <= 512 * 80 || (RULES == kNoRules && in.rows >= 256))
+    launch_top<T, 512, 80 / N, RULES>(in, p, s);
   else
     launch_top<T, 1024, kLong / N, RULES>(in, p, s);
 }

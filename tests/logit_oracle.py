@@ -80,18 +80,23 @@ def lse(x, axis=-1):
         return np.log(np.sum(np.exp(x - low), axis=axis)) + np.squeeze(low, axis)
 
 
-def sum_error(x, tau, threads=256):
+def sum_error(x, tau):
     """Relative error of a kernel's sum of exp((x - max) / tau) over the last
     axis (terms in fp32, -inf ones absent): a term's argument has one rounding
     of the difference, one of the scale 1 / tau and one of the product, the
     hardware exponential is within a step (2 U), and a thread's partial sum of
-    its elements rounds at each addition; partial sums join in 64 bits."""
+    its elements rounds at each addition; partial sums join in 64 bits.  Threads
+    hold whole packs of up to eight elements and one of the row's last: 256 of
+    them or more, 64 in rows of up to 2048 classes, of which at most 64 are
+    entries that the sum leaves out."""
     with np.errstate(all="ignore"):
         d = (np.max(x, axis=-1, keepdims=True) - x) / tau
         e = np.where(np.isfinite(d), np.exp(-np.where(np.isfinite(d), d, 0)), 0.0)
         d = np.where(np.isfinite(d), d, 0.0)
         own = np.sum(e * (3 * d + 4), -1) / np.maximum(np.sum(e, -1), 1e-300)
-        return (own + -(-x.shape[-1] // threads)) * U
+        classes = x.shape[-1] + 64
+        threads = 64 if x.shape[-1] <= 2048 else 256
+        return (own + 8 * -(-classes // (8 * threads)) + 1) * U
 
 
 def top(x, k, tau, last_ties=False):

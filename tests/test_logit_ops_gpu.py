@@ -269,6 +269,52 @@ def test_top_of_many_rows(gpu, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [100, 512, 513, 2047, 2049, 8192, 18710, 20481, 41000])
+def test_top_of_batches(gpu, classes, dtype):
+    """Batches of more than a thousand rows, around the sizes at which a row's
+    workgroup changes."""
+    rng = np.random.default_rng(classes)
+    rows, times = 24, 43
+    x = rows_of(rng, rows, classes, dtype, 1)
+    many = x.repeat(times, 1)
+    for parts in ((), ("bias", "mask"), ("bias", "mask", "history")):
+        kw = make_rules(rng, rows, classes, parts)
+        big = {k: v if k in ("bias", "masks") else np.tile(v, times) for k, v in kw.items() if k != "history_offsets"}
+        if "history" in parts:
+            big["history_offsets"] = np.append(0, np.cumsum(np.tile(np.diff(kw["history_offsets"]), times)))
+        rules = on_device(classes, big) if parts else None
+        y = oracle.rules(f32(x), **kw)
+        for k in (3, 64):
+            values, indices, rest, error = oracle.top(y, k, 1.0)
+            got = gpu.top_logits(many, k, rules)
+            assert np.array_equal(f32(got.values).reshape(times, rows, k), np.broadcast_to(values, (times, rows, k)))
+            assert np.array_equal(got.indices.cpu().numpy().reshape(times, rows, k),
+                                  np.broadcast_to(indices, (times, rows, k)))
+            g = f32(got.rest).astype(np.float64).reshape(times, rows)
+            with np.errstate(invalid="ignore"):
+                assert np.all((np.abs(g - rest) <= error) | (g == rest))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes,first,n", [(512, 0, 512), (512, 100, 77), (2000, 64, 500), (2048, 1000, 1048),
+                                             (6906, 3, 300), (18710, 5000, 700), (40000, 8, 520), (131072, 130000, 500)])
+def test_top_of_a_script(gpu, classes, first, n, dtype):
+    """Only neighbouring classes are allowed: few threads hold candidates, and
+    each of theirs may be among the best."""
+    rng = np.random.default_rng(classes + n)
+    allowed = np.zeros((1, classes), bool)
+    allowed[0, first:first + n] = True
+    for rows in (2, 1030 if classes < 40000 else 260):
+        x = rows_of(rng, 2, classes, dtype)
+        words = ppocr_hip.class_masks(torch.from_numpy(allowed))
+        values, indices, rest, error = oracle.top(oracle.rules(f32(x), masks=words.numpy()), 64, 1.0)
+        got = gpu.top_logits(x.repeat(rows // 2, 1), 64, ppocr_hip.LogitRules(classes, masks=words.cuda()))
+        assert (f32(got.values).reshape(-1, 2, 64) == values).all()
+        assert (got.indices.cpu().numpy().reshape(-1, 2, 64) == indices).all()
+        assert np.all(np.abs(f32(got.rest).reshape(-1, 2) - rest) <= error)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_top_of_rows_with_few_candidates(gpu, dtype):
     x = torch.full((6, 500), -INF, device="cuda")
     x[1, 499] = 2.0
@@ -346,15 +392,17 @@ def test_distill(gpu, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("classes", [301, 6907, 18710, 30000])
-def test_distill_of_many_rows(gpu, classes, dtype):
+@pytest.mark.parametrize("rows,classes", [(600, 301), (600, 6907), (600, 18710), (600, 30000), (1030, 511), (1030, 1999),
+                                          (1030, 2049), (1030, 8193), (1030, 18710)])
+def test_distill_of_many_rows(gpu, rows, classes, dtype):
     """Batches take other workgroups than a few rows do: rows of a batch
     against the plain form."""
     rng = np.random.default_rng(classes)
-    x = rows_of(rng, 600, classes, dtype, 1)
-    values, indices, rest = np.zeros((600, 12), np.float32), np.full((600, 12), -1, np.int32), np.zeros(600, np.float32)
+    x = rows_of(rng, rows, classes, dtype, 1)
+    values, indices = np.zeros((rows, 12), np.float32), np.full((rows, 12), -1, np.int32)
+    rest = np.zeros(rows, np.float32)
     values[:20], indices[:20], rest[:20] = teacher_of(rng, x[:20], 12, 1.5)
-    g = rng.uniform(0.5, 1.5, 600).astype(np.float32)
+    g = rng.uniform(0.5, 1.5, rows).astype(np.float32)
     teacher = ppocr_hip.TopLogits(dev(values), i32(indices), dev(rest))
     loss, grad = gpu.distill(x, teacher, 1.5, dev(g))
     only, state = gpu.distill_loss(x, teacher, 1.5)
