@@ -402,7 +402,9 @@ ppocr_status ppocr_ctc_greedy_decode(const float* steps, size_t time_steps, size
  *
  * Row indices, classes and offsets that the device reads are checked there:
  * those outside their range are left out as described.  Zero rows are no
- * work.  Padding between rows is neither read nor written. */
+ * work.  Padding between rows is neither read nor written.  What a call writes
+ * overlaps nothing else that it is given, but for results in place of the
+ * logits where that is allowed. */
 
 /* `rows` rows of `classes` logits, `stride` elements apart (stride >=
  * classes), each element a float or a bfloat16 by `type`.  1 to 262144
@@ -423,7 +425,8 @@ typedef struct ppocr_logits {
  *
  * history: the classes that each row has emitted, back to back, row r's at
  * history_offsets[r] .. history_offsets[r + 1] - 1 (rows + 1 offsets, within
- * history_len; classes outside the row's are left out).  A class that stands n
+ * history_len; classes outside the row's are left out, and so is what goes past
+ * 2^31 - 1 entries of a row).  A class that stands n
  * > 0 times in it is penalised by the row's repetition (logits above 0 are
  * divided by it, others multiplied), then by frequency * n + presence, which
  * is subtracted.  Null penalties are neutral (1, 0, 0).

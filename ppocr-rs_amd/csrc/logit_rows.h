@@ -367,9 +367,17 @@ __device__ __forceinline__ float apply_rules(const RowRules& r, float x, int c, 
 __device__ __forceinline__ void count_history(const RowRules& r, int first, int n, int* counts) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < r.n_history; i += blockDim.x) {
-    const int c = r.history[i] - first;
-    if (c >= 0 && c < n) atomicAdd(&counts[c], 1);
+  // Four entries a thread are on their way at once.
+  for (unsigned i = threadIdx.x; i < (unsigned)r.n_history; i += 4 * blockDim.x) {
+    int c[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned at = i + q * blockDim.x;
+      c[q] = at < (unsigned)r.n_history ? r.history[at] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c[q] >= first && c[q] < first + n) atomicAdd(&counts[c[q] - first], 1);
   }
   __syncthreads();
 }

@@ -12,7 +12,7 @@ constexpr int kThreads = 256, kChunk = 4096;
 // history's classes in the chunk are an LDS histogram, so a chunk costs one
 // pass over the row's history (from L2 after the first chunk).  2560 x 6906 fp32
 // under line masks and a bias: 19 us; 256 x 131072 bf16 under masks and
-// histories of up to 2000 classes: 27 us, 18 of them its bytes.
+// histories of up to 2000 classes: 25 us, 18 of them its bytes.
 template <typename T, bool HISTORY>
 __global__ __launch_bounds__(kThreads) void logit_rules_kernel(LogitRows in, RuleParams p, T* out, int64_t out_stride,
                                                                int chunk) {

@@ -172,6 +172,24 @@ def test_a_long_history_of_one_class(gpu):
     assert np.array_equal(f32(top.values), values) and np.array_equal(top.indices.cpu().numpy(), indices)
 
 
+def test_a_history_past_32_bits(gpu):
+    """Offsets beyond 2^31 entries, and a row with more entries than an int
+    counts: those past 2^31 - 1 are left out."""
+    n = (1 << 31) + 5000
+    history = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    history[:3] = torch.tensor([0, 1, 1])
+    history[(1 << 31) - 2] = 2  # the last of a row's entries that count
+    history[(1 << 31) - 1:] = 3
+    x = torch.zeros((2, 8), device="cuda")
+    for offsets, want in (([0, n, n], [[-1, -2, -1, 0, 0, 0, 0, 0], [0] * 8]),
+                          ([5, 9, n], [[0] * 8, [0, 0, -1, -9, 0, 0, 0, 0]]),
+                          ([n - 7, n, n], [[0, 0, 0, -7, 0, 0, 0, 0], [0] * 8])):
+        rules = ppocr_hip.LogitRules(8, history=history, frequency=torch.ones(2, device="cuda"),
+                                     history_offsets=torch.tensor(offsets, device="cuda"))
+        assert gpu.logit_rules(x, rules).tolist() == want
+    assert gpu.top_logits(x, 8, rules).values.tolist() == [[0] * 7 + [-7], [0] * 8]
+
+
 # ----------------------------------------------------------------------- top
 
 def check_top(gpu, x, k, tau, kw=None):
