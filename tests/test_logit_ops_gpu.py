@@ -727,6 +727,29 @@ def test_host_memory_is_refused_and_the_next_call_works(gpu):
         assert torch.equal(gpu.logit_rules(x, rules), x)
 
 
+def test_results_that_are_not_asked_for(gpu):
+    """The C calls without a rest or a state, and rules without any part."""
+    rng = np.random.default_rng(23)
+    x = rows_of(rng, 6, 6906, "f32")
+    lib, rows = ppocr_hip.lib(), ppocr_hip._rows(x, "logits")
+    top = gpu.top_logits(x, 5)
+    values, indices = torch.zeros_like(top.values), torch.zeros_like(top.indices)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.ppocr_hip_top_logits(gpu.handle, rows, None, 5, 1.0, values.data_ptr(), indices.data_ptr(), None, stream) == 0
+    assert torch.equal(values, top.values) and torch.equal(indices, top.indices)
+    student = rows_of(rng, 6, 6906, "f32")
+    want, _ = gpu.distill_loss(student, top)
+    loss = torch.zeros_like(want)
+    teacher = ppocr_hip._Teacher(top.values.data_ptr(), top.indices.data_ptr(), top.rest.data_ptr(), 5)
+    assert lib.ppocr_hip_distill_loss(gpu.handle, ppocr_hip._rows(student, "student"), teacher, 1.0, loss.data_ptr(), None,
+                                      stream) == 0
+    assert torch.equal(loss, want)
+    none = ppocr_hip.LogitRules(6906)
+    assert torch.equal(gpu.logit_rules(x, none), x)
+    again = gpu.top_logits(x, 5, none)
+    assert torch.equal(again.values, top.values) and torch.equal(again.rest, top.rest)
+
+
 def test_the_callers_device_stays_current(gpu):
     x = torch.randn(2, 40, device="cuda")
     gpu.top_logits(x, 3)
