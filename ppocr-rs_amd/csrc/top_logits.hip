@@ -45,9 +45,9 @@ enum RuleParts { kNoRules, kTables, kHistory };
 // The penalties on a part in registers.  The history is counted in windows of
 // classes, whole rounds of packs of a part; the row's last classes have counters
 // of their own behind the window's.  Short rows take small windows, which leave
-// LDS for more workgroups (10000 x 6906 fp32, top 8: 122 us against 143 in one
-// window, 20000 x 300 56 against 188), long ones large windows, for each of which
-// the history is read again (2560 x 18710: 83 us against 88 in windows of 4096).
+// LDS for more workgroups (10000 x 6906 fp32, top 8: 102 us against 112 in one
+// window), long ones large windows, for each of which the history is read again
+// (2560 x 18710: 83 us against 88 in windows of 4096).
 constexpr int history_window(int part_classes) {
   return part_classes <= 2048 ? part_classes : part_classes <= 8192 ? 4096 : 8192;
 }
@@ -121,7 +121,7 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
 // workgroup, the row read once (parts of longer rows a second time).  fp32 rows
 // are bound by HBM (10240 x 18710, top 8: 133 us, 5.8 TB/s), bf16 ones and long
 // lists by vector work, some 1000 to 1700 operations a wave, a third of them
-// exponentials (the same in bf16, top 8: 94 us, top 64: 128 us, where HBM would
+// exponentials (the same in bf16, top 8: 86 us, top 64: 122 us, where HBM would
 // take 70).
 //
 // The classes form groups, each with its best (logit, first place that holds
@@ -160,6 +160,27 @@ struct TopShared {
 template <int NT, int N>
 constexpr int top_list() {
   return NT == 1024 && N == 4 ? 256 : 512;
+}
+// Its distance to the next wave's, so that the lists' like places lie in
+// different banks.
+template <int NT, int N>
+constexpr int list_stride() {
+  return top_list<NT, N>() + (NT > 64 ? 4 : 0);
+}
+
+// Where the history's counters lie, in entries of the lists: behind them where a
+// row may have several parts, else in their place, since the counting is done
+// when the lists begin.
+template <int NT, int N>
+constexpr int history_at() {
+  return NT == 1024 ? NT / 64 * list_stride<NT, N>() : 0;
+}
+template <int NT, int PER, int N, RuleParts RULES>
+constexpr size_t top_lds() {
+  const size_t lists = NT / 64 * list_stride<NT, N>() * sizeof(uint64_t);
+  const size_t counts =
+      history_at<NT, N>() * sizeof(uint64_t) + (history_window(NT * PER * N) + 8) * sizeof(int);
+  return RULES == kHistory && counts > lists ? counts : lists;
 }
 
 // Bound of the list: the composite (value key, ~place) that at least k of the
@@ -264,10 +285,10 @@ constexpr int top_waves() {
 
 template <typename T, int NT, int PER, RuleParts RULES>
 __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logits_kernel(LogitRows in, TopParams p, int parts) {
-  constexpr int N = Pack<T>::N, W = NT / 64, kList = top_list<NT, N>();
+  constexpr int N = Pack<T>::N, W = NT / 64, kList = top_list<NT, N>(), kStride = list_stride<NT, N>();
   __shared__ TopShared<NT> sh;
-  extern __shared__ __align__(16) uint64_t lists[];  // [W][kList], then the history's counters
-  int* counts = reinterpret_cast<int*>(lists + W * kList);
+  extern __shared__ __align__(16) uint64_t lists[];  // [W][kStride]
+  int* counts = reinterpret_cast<int*>(lists + history_at<NT, N>());
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(in.x) + row * in.stride;
@@ -351,7 +372,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
   // Classes above the bound go to the wave's list; the others' sums.
   const float floor_value = key_value(bound);
   const uint32_t floor_place = (uint32_t)bound;
-  uint64_t* list = lists + wave * kList;
+  uint64_t* list = lists + wave * kStride;
   float wm = -INFINITY;
   double ws = 0.0;
   int n_wave = 0;
@@ -364,10 +385,10 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     // A class passes above the bound's value, or at it in a place that the
     // bound reaches; at least -FLT_MAX in any case.
     const auto take = [&](float v, int at, int cls) {
-      uint64_t lanes = lanes_where(v >= floor_value);
-      if (!lanes) return false;
-      if (floor_place) lanes &= lanes_where(v > floor_value) | lanes_where((uint32_t)~at >= floor_place);
-      const bool mine = lanes >> lane & 1;
+      bool mine = v >= floor_value;
+      if (!lanes_where(mine)) return false;
+      if (floor_place) mine = mine && (v > floor_value || (uint32_t)~at >= floor_place);
+      const uint64_t lanes = lanes_where(mine);
       const int slot = __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, n_wave));
       if (mine) list[min(slot, kList - 1)] = (uint64_t)number_key(v) << 32 | (uint32_t)(p.last_ties ? cls : ~cls);
       n_wave += __popcll(lanes);
@@ -404,24 +425,33 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
     join_sums(wm, ws, fminf(m, FLT_MAX), sum, c);
   }
   if (lane == 0) sh.wave_max[wave] = wm, sh.wave_sum[wave] = ws, sh.count[wave] = n_wave;
-  // Zeros behind the list, to the next eight.
-  if (lane < 8 && n_wave + lane < kList) list[n_wave + lane] = 0;
+  // Zeros behind the list, to the next step of the ranking.
+  constexpr int kStep = W > 1 ? 4 : 8;
+  if (lane < kStep && n_wave + lane < kList) list[n_wave + lane] = 0;
   __syncthreads();
 
-  int n = 0, most = 0;
+  int n = 0, most = 0, ends[W];
 #pragma unroll
-  for (int w = 0; w < W; ++w) n += sh.count[w], most = max(most, sh.count[w]);
+  for (int w = 0; w < W; ++w) ends[w] = n += sh.count[w], most = max(most, sh.count[w]);
   if (n <= kSorted && most <= kList && !sh.nan) {
-    for (int i = tid; i < n; i += NT) {
-      int from = 0, at = i;
-      while (at >= sh.count[from]) at -= sh.count[from++];
-      const uint64_t key = lists[from * kList + at];
-      int rank = 0;
-      for (int w = 0; w < W; ++w)
-        for (int o = 0; o < sh.count[w]; o += 8)
+    // W lanes a class, each with one list (10240 x 6906 fp32 under masks, top 8:
+    // 67 us against 78 with a lane for all lists, 1 x 18710, top 5: 6.4 against 7.5).
+    constexpr int kUnroll = W > 1 ? 1 : 2;
+    for (int i = tid / W; i < n; i += 64) {
+      int at = i;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) rank += lists[w * kList + o + q] > key;
-      sh.sorted[rank] = key;
+      for (int w = 0; w + 1 < W; ++w) at = i >= ends[w] ? (w + 1) * kStride + i - ends[w] : at;
+      const uint64_t key = lists[at];
+      const uint64_t* mine = lists + tid % W * kStride;
+      const int end = sh.count[tid % W];
+      int rank = 0;
+#pragma unroll kUnroll
+      for (int o = 0; o < end; o += kStep)
+#pragma unroll
+        for (int q = 0; q < kStep; ++q) rank += mine[o + q] > key;
+#pragma unroll
+      for (int o = 1; o < W; o <<= 1) rank += __shfl_xor(rank, o);
+      if (tid % W == 0) sh.sorted[rank] = key;
     }
   } else {
     search_row<T, RULES, NT, history_window(NT * PER * N)>(x, r, in.classes, p, c, counts, sh, wm, ws);
@@ -466,8 +496,7 @@ __global__ __launch_bounds__(NT, (top_waves<T, NT, PER, RULES>())) void top_logi
 template <typename T, int NT, int PER, RuleParts RULES>
 void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
   constexpr int kClasses = NT * PER * Pack<T>::N;
-  const size_t lds = (size_t)NT / 64 * top_list<NT, Pack<T>::N>() * sizeof(uint64_t) +
-                     (RULES == kHistory ? (history_window(kClasses) + 8) * sizeof(int) : 0);
+  constexpr size_t lds = top_lds<NT, PER, Pack<T>::N, RULES>();
   hipLaunchKernelGGL((top_logits_kernel<T, NT, PER, RULES>), dim3((unsigned)in.rows), dim3(NT), lds, s, in, p,
                      (in.classes + kClasses - 1) / kClasses);
 }
@@ -482,7 +511,7 @@ void launch_top(const LogitRows& in, const TopParams& p, hipStream_t s) {
 // top 64: 149 us against 223 with 512).  Longer rows are read twice in parts
 // rather than held by 1024 threads, whose one workgroup leaves its CU idle at
 // each wait (700 x 70000 fp32: 52 us against 57, 1500 x 30001 in one part 42
-// against 80), but where rules would be applied twice too (256 x 131072 under
+// against 80 then, 37 now), but where rules would be applied twice too (256 x 131072 under
 // masks 37 against 54) or few rows leave CUs idle.
 template <typename T, RuleParts RULES>
 void launch_top_rules(const LogitRows& in, const TopParams& p, hipStream_t s) {
