@@ -293,26 +293,39 @@ def _torch():
 
 
 def _current_stream(device):
-    """The HIP stream that torch uses on the device."""
-    return _torch_module.cuda.current_stream(device).cuda_stream
+    """The HIP stream that torch uses on the device (torch.cuda.current_stream
+    makes an object of it first, a microsecond of a small call's ten)."""
+    return _torch_module._C._cuda_getCurrentRawStream(device)
 
 
 _ROW_TYPES = {"torch.float32": 0, "torch.bfloat16": 1}
+_type_names = {}
+
+
+def _type_name(t):
+    """``str(t.dtype)``, formed once a type."""
+    name = _type_names.get(t.dtype)
+    if name is None:
+        name = _type_names[t.dtype] = str(t.dtype)
+    return name
 
 
 def _rows(t, what):
     """``ppocr_logits`` of a tensor [..., classes] whose rows lie one stride apart."""
-    if t.dim() < 1:
-        raise ValueError(f"{what} needs a dimension of classes")
-    if t.dim() != 2:
-        t = t.view(-1, t.shape[-1])  # raises where the rows are not one stride apart
-    rows, classes = t.shape
-    if classes > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2:
+        if not shape:
+            raise ValueError(f"{what} needs a dimension of classes")
+        t = t.view(-1, shape[-1])  # raises where the rows are not one stride apart
+        shape = t.shape
+    rows, classes = shape
+    stride, step = t.stride()
+    if classes > 1 and step != 1:
         raise ValueError(f"{what}: the classes of a row must be adjacent")
-    kind = _ROW_TYPES.get(str(t.dtype))
+    kind = _ROW_TYPES.get(_type_name(t))
     if kind is None:
         raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}")
-    return _Logits(t.data_ptr(), rows, classes, t.stride(0) if rows > 1 else max(classes, t.stride(0)), kind)
+    return _Logits(t.data_ptr(), rows, classes, stride if rows > 1 else max(classes, stride), kind)
 
 
 def _rows_like(t, like, what):
@@ -321,10 +334,10 @@ def _rows_like(t, like, what):
     return _rows(t, what)
 
 
-def _output(torch, out, like, rows):
+def _output(out, like, rows):
     """The rows that a call writes and their stride: given, or new ones."""
     if out is None:
-        return torch.empty_like(like, memory_format=torch.contiguous_format), rows.classes
+        return like.new_empty(like.shape), rows.classes
     return out, _rows_like(out, like, "out").stride
 
 
@@ -332,7 +345,7 @@ def _packed(t, dtype, count, what):
     """Pointer of a contiguous tensor of ``count`` elements (None: None)."""
     if t is None:
         return None
-    if str(t.dtype) != "torch." + dtype or not t.is_contiguous():
+    if _type_name(t) != "torch." + dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
     if count is not None and t.numel() != count:
         raise ValueError(f"{what} has {t.numel()} elements, needs {count}")
@@ -352,9 +365,10 @@ class TopLogits:
 
 
 def _teacher(t, rows):
-    if t.values.dim() < 1 or t.values.shape != t.indices.shape:
+    shape = t.values.shape
+    if not shape or shape != t.indices.shape:
         raise ValueError("the teacher's values and indices must have one shape [..., k]")
-    k = t.values.shape[-1]
+    k = shape[-1]
     return _Teacher(_packed(t.values, "float32", rows * k, "the teacher's values"),
                     _packed(t.indices, "int32", rows * k, "the teacher's indices"),
                     _packed(t.rest, "float32", rows, "the teacher's rest"), k)
@@ -489,10 +503,10 @@ class Gpu:
     def logit_rules(self, logits, rules, out=None):
         """Penalties, biases and masks of ``rules`` (LogitRules) on logits
         [..., classes] (float32 or bfloat16); ``out`` may be the logits."""
-        torch = _torch()
+        _torch()
         rows = _rows(logits, "logits")
         rules.check(rows.rows)
-        out, stride = _output(torch, out, logits, rows)
+        out, stride = _output(out, logits, rows)
         _check(_lib.ppocr_hip_logit_rules(self.handle, rows, rules.struct, out.data_ptr(), stride,
                                           _current_stream(self.device)))
         return out
@@ -505,9 +519,9 @@ class Gpu:
         if rules is not None:
             rules.check(rows.rows)
         lead = logits.shape[:-1]
-        values = torch.empty((*lead, int(k)), dtype=torch.float32, device=logits.device)
-        indices = torch.empty((*lead, int(k)), dtype=torch.int32, device=logits.device)
-        rest = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        values = logits.new_empty((*lead, int(k)), dtype=torch.float32)
+        indices = logits.new_empty((*lead, int(k)), dtype=torch.int32)
+        rest = logits.new_empty(lead, dtype=torch.float32)
         _check(_lib.ppocr_hip_top_logits(self.handle, rows, rules.struct if rules is not None else None, int(k),
                                          temperature, values.data_ptr(), indices.data_ptr(), rest.data_ptr(),
                                          _current_stream(self.device)))
@@ -520,8 +534,8 @@ class Gpu:
         rows = _rows(student, "student")
         t = _teacher(teacher, rows.rows)
         lead = student.shape[:-1]
-        loss = torch.empty(lead, dtype=torch.float32, device=student.device)
-        state = torch.empty((*lead, 4), dtype=torch.float32, device=student.device)
+        loss = student.new_empty(lead, dtype=torch.float32)
+        state = student.new_empty((*lead, 4), dtype=torch.float32)
         _check(_lib.ppocr_hip_distill_loss(self.handle, rows, t, temperature, loss.data_ptr(), state.data_ptr(),
                                            _current_stream(self.device)))
         return loss, state
@@ -529,10 +543,10 @@ class Gpu:
     def distill_grad(self, student, teacher, state, temperature=1.0, grad_loss=None, out=None):
         """Gradient of ``sum(grad_loss * loss)`` by the student's logits, from
         the state that ``distill_loss`` left; ``out`` may be the logits."""
-        torch = _torch()
+        _torch()
         rows = _rows(student, "student")
         t = _teacher(teacher, rows.rows)
-        out, stride = _output(torch, out, student, rows)
+        out, stride = _output(out, student, rows)
         _check(_lib.ppocr_hip_distill_grad(self.handle, rows, t, _packed(state, "float32", rows.rows * 4, "state"),
                                            temperature, _packed(grad_loss, "float32", rows.rows, "grad_loss"),
                                            out.data_ptr(), stride, _current_stream(self.device)))
@@ -544,8 +558,8 @@ class Gpu:
         torch = _torch()
         rows = _rows(student, "student")
         t = _teacher(teacher, rows.rows)
-        loss = torch.empty(student.shape[:-1], dtype=torch.float32, device=student.device)
-        out, stride = _output(torch, out, student, rows)
+        loss = student.new_empty(student.shape[:-1], dtype=torch.float32)
+        out, stride = _output(out, student, rows)
         _check(_lib.ppocr_hip_distill(self.handle, rows, t, temperature,
                                       _packed(grad_loss, "float32", rows.rows, "grad_loss"), loss.data_ptr(),
                                       out.data_ptr(), stride, _current_stream(self.device)))
