@@ -333,6 +333,24 @@ def test_top_of_a_script(gpu, classes, first, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [9, 6906, 18710, 30001])
+def test_top_under_biases_that_are_no_numbers(gpu, classes, dtype):
+    """Infinite biases and NaN at the table's start and end reach their own
+    classes alone, and not those that the mask takes."""
+    rng = np.random.default_rng(classes)
+    x = rows_of(rng, 6, classes, dtype)
+    bias = rng.normal(size=(3, classes)).astype(np.float32)
+    bias[0, :8], bias[1, :8], bias[2, :8] = np.nan, INF, -INF
+    bias[0, -1], bias[1, -1], bias[2, -1] = INF, -INF, np.nan
+    allowed = rng.random((2, classes)) < 0.5
+    allowed[:, :8], allowed[:, -1] = [[False], [True]], [False, True]
+    masks = ppocr_hip.class_masks(torch.from_numpy(allowed)).numpy()
+    rows = dict(row_bias=np.array([0, 1, 2, 0, 1, 2], np.int32))
+    for kw in (dict(bias=bias, **rows), dict(bias=bias, masks=masks, row_mask=np.array([0, 0, 0, 1, 1, 1], np.int32), **rows)):
+        check_top(gpu, x, 20, 1.0, kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_top_of_rows_with_few_candidates(gpu, dtype):
     x = torch.full((6, 500), -INF, device="cuda")
     x[1, 499] = 2.0
