@@ -132,9 +132,8 @@ __device__ __forceinline__ void read_part(P& d, const T* x, const RowRules& r, c
 // The k best classes of a row and the log-sum-exp of the others, one row a
 // workgroup, the row read once (parts of longer rows a second time).  fp32 rows
 // are bound by HBM (10240 x 18710, top 8: 133 us, 5.8 TB/s), bf16 ones and long
-// lists by vector work, some 1000 to 1700 operations a wave, a third of them
-// exponentials (the same in bf16, top 8: 86 us, top 64: 122 us, where HBM would
-// take 70).
+// lists by vector work (the same in bf16, top 8: 86 us, top 64: 122 us at 1450
+// operations a wave, 80% busy, where HBM would take 70).
 //
 // The classes form groups, each with its best (logit, first place that holds
 // it).  The k-th best group bounds the k-th best class from below, and only
